@@ -45,7 +45,9 @@ typedef struct qph_ctx qph_ctx;
 QPH_API int qph_ctx_create(int device, qph_ctx** out);
 QPH_API int qph_ctx_destroy(qph_ctx* ctx);
 /* Use an external HIP stream (e.g. a framework's current stream) instead of
- * the context's own; NULL restores the context's stream. */
+ * the context's own; NULL restores the context's stream, and
+ * QPH_STREAM_DEFAULT takes HIP's default (null) stream. */
+#define QPH_STREAM_DEFAULT ((void*)1)
 QPH_API int qph_ctx_set_stream(qph_ctx* ctx, void* hip_stream);
 QPH_API void* qph_ctx_stream(qph_ctx* ctx);
 /* Bytes of device scratch the context has allocated for standalone operator
@@ -306,6 +308,113 @@ QPH_API int qph_pack_crops(qph_ctx* ctx, int32_t n, const uint8_t* const* crops,
  * (1, 1), out-of-range samples ignored. */
 QPH_API int qph_db_mask(qph_ctx* ctx, const float* pred, int64_t h, int64_t w, float thresh,
                         int32_t dilate, uint8_t* mask);
+
+/* ----------------------------- 4-bit weights and key / value caches */
+
+/* Operators of a decoder that writes its text token by token: its linears run
+ * over a few rows and read every weight for each token, its attention reads
+ * the whole cache of keys and values.  Both are held in 4 bits.  No
+ * counterpart in the reference, whose recogniser is CTC only.
+ *
+ * Format: 32 neighbouring elements share a scale byte s.  An element is a code
+ * of four bits, a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6, and stands for
+ * that number times 2^(s - 127).  s = 255 marks a block that held a NaN or an
+ * infinity; all its elements read as NaN.  Two codes a byte, the even element
+ * in the low four bits.  Quantising takes the smallest power of two, at least
+ * 2^-100 and at most 2^125, that puts the block's largest magnitude at 6 or
+ * below, and rounds to nearest, ties to the even code: an element is off by
+ * at most the block's scale, 2^(s - 127), unless the largest lies past 6 *
+ * 2^125 (then it is held as that).  Callers may bring their own blocks with
+ * scale bytes 27 to 252 and 255.
+ *
+ * These calls take float32, float16 or bfloat16 (dtype; weights are
+ * quantised from any of them) and accumulate in float32.  They allocate
+ * nothing, keep nothing between calls, and may be recorded into a graph. */
+#define QPH_F32 0
+#define QPH_F16 1
+#define QPH_BF16 2
+
+/* Weight rows to 4 bits: element (r, i) at x[r * row_stride + i * col_stride]
+ * (elements), i < k.  With kp = k rounded up to 128: codes [rows][kp / 2]
+ * (16-byte aligned), scales [rows][kp / 32] (4-byte aligned); elements past k
+ * are zero. */
+QPH_API int qph_quantize4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t rows, int64_t k,
+                          int64_t row_stride, int64_t col_stride, void* codes, void* scales);
+/* The linear over such weights: y[rows, n] = act(x[rows, k] W^T + bias[n]) +
+ * residual[rows, n], W [n][kp] as qph_quantize4 leaves it.  x, bias, residual
+ * and y are of dtype; x has rows x_stride elements apart, y and residual are
+ * contiguous (residual may be y); bias, act and residual may be NULL.  The
+ * products are exact, sums are float32, y is rounded once.  GELU uses the
+ * error function itself, not the approximation of qph_linear. */
+QPH_API int qph_linear4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t x_stride,
+                        const void* codes, const void* scales, const void* bias, int64_t rows,
+                        int64_t k, int64_t n, const qph_act* act, const void* residual, void* y);
+
+/* A paged cache: a pool of n_pages pages of page_size tokens (a power of two,
+ * 16 to 32768), each with `heads` keys and values of dh elements (32, 64, 96,
+ * 128, 192 or 256).  Codes [n_pages][heads][page_size][dh / 2] bytes (16-byte
+ * aligned), scales [n_pages][heads][page_size][dh / 32].  A token's slot is
+ * page * page_size + its place in the page. */
+typedef struct {
+  void *k_codes, *k_scales, *v_codes, *v_scales;
+  int64_t n_pages;
+  int32_t page_size, heads, dh;
+} qph_cache4;
+
+/* Quantises tokens' keys and values into their slots: k, v [tokens][heads][dh]
+ * with strides {token, head} in elements, dh contiguous.  A slot outside the
+ * pool (a padded token's -1) is skipped.  The slots of one call must differ
+ * from each other: of tokens with the same slot, what is stored there may be
+ * a mixture (nothing else is touched). */
+QPH_API int qph_cache4_write(qph_ctx* ctx, const qph_cache4* cache, const void* k, const void* v,
+                             int32_t dtype, int64_t tokens, const int64_t k_strides[2],
+                             const int64_t v_strides[2], const int64_t* slots);
+/* The tokens of any slots back as dense rows; zeros for a slot outside the
+ * pool. */
+QPH_API int qph_cache4_read(qph_ctx* ctx, const qph_cache4* cache, void* k, void* v, int32_t dtype,
+                            int64_t tokens, const int64_t k_strides[2], const int64_t v_strides[2],
+                            const int64_t* slots);
+
+/* Attention of new tokens over cached keys and values (the new tokens' own are
+ * written first).  Sequence b has lens[b] cached tokens, token j of it at place
+ * j % page_size of page page_table[b * table_stride + j / page_size]; its new
+ * tokens are q[starts[b] .. starts[b + 1] - 1], or with starts NULL max_new
+ * tokens each in order, and are the last ones of the sequence: the i-th of n
+ * stands at position p = lens[b] - n + i.  It sees the keys j < lens[b] with
+ * j <= p (causal), j > p - window (window > 0), on pages of the pool (a page
+ * number outside it holds no keys).  Query head h reads the cache's head
+ * h / (heads / cache heads).
+ *   out = sum_j softmax_j(scale q . k_j) v_j
+ *   lse = log sum_j exp(scale q . k_j)     (float32 [tokens][heads], or NULL)
+ * A row that sees no key gets zeros and -infinity.  Rows that no sequence has
+ * are left as they were.  max_new and max_len (host) bound the sequences' new
+ * and cached tokens; they choose the work's split, and longer ones only run
+ * slower.  lens are cut at max_pages pages.  Scores, sums and the running
+ * maximum are float32, keys and values exact, the probabilities kept to 16
+ * bits (24 for float32) in the second product.
+ * page_table, lens and starts are device memory.  The workspace (device, of
+ * qph_attention_cache4_workspace bytes for the same arguments, which depend on
+ * no device data) is this call's until it has run; calls that may overlap need
+ * one each. */
+typedef struct {
+  const void* q;              /* [tokens][heads][dh], strides {token, head} */
+  void* out;                  /* the same shape */
+  float* lse;
+  int64_t q_strides[2], out_strides[2];
+  int64_t tokens, batch;
+  const int32_t* page_table;
+  int64_t table_stride, max_pages;
+  const int32_t* lens;        /* [batch] */
+  const int32_t* starts;      /* [batch + 1], not decreasing, or NULL */
+  int32_t dtype, heads, max_new, max_len;
+  float scale;                /* finite, not 0 */
+  int32_t causal, window;     /* window 0: none */
+  void* workspace;
+  size_t workspace_bytes;
+} qph_attn4;
+QPH_API int qph_attention_cache4_workspace(const qph_cache4* cache, const qph_attn4* args,
+                                           size_t* bytes);
+QPH_API int qph_attention_cache4(qph_ctx* ctx, const qph_cache4* cache, const qph_attn4* args);
 
 /* ------------------------------------------------------------- session */
 

@@ -24,6 +24,8 @@ RUN_UPLOAD, RUN_DOWNLOAD = 1, 2
 NET_SEPARATE_LAUNCHES = 1
 NET_FUSED_HEAD = 2
 NOALLOC_WK_FLOATS = 1 << 20
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+STREAM_DEFAULT = 1
 
 I64 = ctypes.c_int64
 I64_4 = I64 * 4
@@ -78,6 +80,21 @@ class PlanSpec(ctypes.Structure):
                 ("out_numel", ctypes.POINTER(I64))]
 
 
+class Cache4(ctypes.Structure):
+    """qph_cache4: a paged 4-bit cache's memory and shape."""
+    _fields_ = [("k_codes", P), ("k_scales", P), ("v_codes", P), ("v_scales", P),
+                ("n_pages", I64), ("page_size", I32), ("heads", I32), ("dh", I32)]
+
+
+class Attn4(ctypes.Structure):
+    """qph_attn4: the arguments of the attention over a 4-bit cache."""
+    _fields_ = [("q", P), ("out", P), ("lse", P), ("q_strides", I64 * 2), ("out_strides", I64 * 2),
+                ("tokens", I64), ("batch", I64), ("page_table", P), ("table_stride", I64),
+                ("max_pages", I64), ("lens", P), ("starts", P), ("dtype", I32), ("heads", I32),
+                ("max_new", I32), ("max_len", I32), ("scale", F32), ("causal", I32),
+                ("window", I32), ("workspace", P), ("workspace_bytes", ctypes.c_size_t)]
+
+
 # exported symbol -> (argtypes, restype); every symbol include/qppocr_hip.h declares
 SIGNATURES = {
     "qph_ctx_create": ([ctypes.c_int, ctypes.POINTER(P)], ctypes.c_int),
@@ -126,6 +143,14 @@ SIGNATURES = {
     "qph_resize_nearest": ([P, P, I64, I64, I64, I64, I64, P], ctypes.c_int),
     "qph_binary_inplace": ([P, P, P, I64, I64, I32, I32], ctypes.c_int),
     "qph_reduce_mean_last": ([P, P, I64, I64, P], ctypes.c_int),
+    "qph_quantize4": ([P, P, I32, I64, I64, I64, I64, P, P], ctypes.c_int),
+    "qph_linear4": ([P, P, I32, I64, P, P, P, I64, I64, I64, ctypes.POINTER(Act), P, P],
+                    ctypes.c_int),
+    "qph_cache4_write": ([P, ctypes.POINTER(Cache4), P, P, I32, I64, P, P, P], ctypes.c_int),
+    "qph_cache4_read": ([P, ctypes.POINTER(Cache4), P, P, I32, I64, P, P, P], ctypes.c_int),
+    "qph_attention_cache4_workspace": ([ctypes.POINTER(Cache4), ctypes.POINTER(Attn4),
+                                        ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "qph_attention_cache4": ([P, ctypes.POINTER(Cache4), ctypes.POINTER(Attn4)], ctypes.c_int),
     "qph_net_create": ([P, ctypes.POINTER(NetSpec), ctypes.POINTER(P), ctypes.POINTER(P)],
                        ctypes.c_int),
     "qph_net_destroy": ([P], ctypes.c_int),

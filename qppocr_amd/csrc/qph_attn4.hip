@@ -1,0 +1,611 @@
+// Attention over the 4-bit key / value cache (format: qph_fp4.h).
+//
+// For a new token at position p of its sequence and a query head of the
+// cache's head h, over the visible keys j:
+//   s_j = scale q . k_j,  m = max s_j,  o = sum exp(s_j - m) v_j / sum exp(s_j - m)
+// in one pass over the cache with a running m (the sums so far are multiplied
+// by exp(m_old - m_new) when it grows).
+//
+// A wave holds 16 NQ rows (a row is one new token and one query head of h) as
+// the columns of its MFMAs and walks the keys in tiles of 32:
+//   S^T [16 keys][16 rows] = K [16][32 d] Q^T [32 d][16]   (D: lane's row, 4 keys)
+//   O^T [16 d][16 rows]   += V^T [16 d][32 keys] P^T [32 keys][16]
+// The sum over keys (or d) inside an MFMA may take them in any order that both
+// operands share, and both orders are chosen so that nothing moves between
+// lanes: lane group g holds, of a 32-key tile, the keys 4 g .. 4 g + 3 and
+// 16 + 4 g .. 16 + 4 g + 3, which are those of its four S values of either
+// half, so exp(s - m) is the second product's operand where it stands; and it
+// reads dh / 4 neighbouring d of a key, W = dh / 32 words of codes.  Of a
+// value row lane i reads bytes W i .. W i + W - 1, the 2 W elements d = 2 W i + m
+// that become row i of product m.  Codes turn into bfloat16 in registers, one
+// instruction for two.
+#include <algorithm>
+#include <cmath>
+
+#include "qph_fp4.h"
+
+namespace qph {
+
+struct Attn4 {
+  const unsigned char *kc, *ks, *vc, *vs;
+  int64_t n_pages;
+  int shift;
+  int heads, group;               // the cache's heads, query heads to each
+  const void* q;
+  void* out;
+  float* lse;                     // [tokens][heads * group], or NULL
+  int64_t qt, qh, ot, oh;         // strides of a token and a head
+  int64_t tokens;
+  int batch;
+  const int32_t* table;
+  int64_t table_stride;
+  int max_pages;
+  const int32_t* lens;
+  const int32_t* starts;          // or NULL: `news` tokens a sequence
+  int news;
+  float scale;
+  int causal, window;
+  int row_tiles, splits;          // grid: row tiles x splits x heads x batch
+  int64_t chunk;                  // keys a split
+  float* part_o;                  // [split][token][query head][dh], splits > 1
+  float* part_ml;                 // [split][token][query head][2]
+};
+
+constexpr int64_t kMaxKeys = 0x7fffff00;     // of one sequence: positions stay in 31 bits
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The larger over the four lanes of one column (lane ^ 16, lane ^ 32).
+__device__ __forceinline__ float column_max(float v) {
+  u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+__device__ __forceinline__ float column_sum(float v) {
+  u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// W words a lane: dh = 32 W.
+template <int W>
+struct Lane {
+  static constexpr bool straddle = W == 3 || W == 6;   // a lane's bytes lie in two blocks
+  static constexpr int vwords = (W + 3) / 4;           // words that hold W bytes
+};
+
+template <typename E, int W, int NQ, int WS>
+__global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
+  constexpr int T = E::terms, PT = T < 2 ? 2 : T;
+  constexpr int DH = 32 * W;
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int li = lane & 15, kg = lane >> 4;
+  unsigned id = blockIdx.x;
+  const int rt0 = id % a.row_tiles; id /= a.row_tiles;
+  const int split = id % a.splits; id /= a.splits;
+  const int h = id % a.heads;
+  const int b = id / a.heads;
+
+  // this sequence's new tokens and cached keys, inside what the caller's
+  // buffers hold whatever the device arrays say
+  int64_t t0, t1;
+  if (a.starts) {
+    t0 = min(max((int64_t)a.starts[b], (int64_t)0), a.tokens);
+    t1 = min(max((int64_t)a.starts[b + 1], t0), a.tokens);
+  } else {
+    t0 = (int64_t)b * a.news;
+    t1 = t0 + a.news;
+  }
+  const int news = (int)(t1 - t0);
+  const int room = (int)min((int64_t)a.max_pages << a.shift, kMaxKeys);
+  const int len = min(max(a.lens[b], 0), room);
+  const int64_t rows = (int64_t)news * a.group;
+  const int32_t* table = a.table + b * a.table_stride;
+  const int first = len - news;          // position of the first new token
+  const int base = a.window > 0 ? max(0, first - a.window + 1) & ~31 : 0;
+  const int from = (int)min(base + split * a.chunk, (int64_t)room);
+  const int to = split == a.splits - 1 ? room : (int)min(from + a.chunk, (int64_t)room);
+
+  for (int64_t tile = WS == 4 ? rt0 : (int64_t)rt0 * 4 + wave; tile * 16 * NQ < rows;
+       tile += (int64_t)a.row_tiles * (WS == 4 ? 1 : 4)) {
+    // (a row has seen a key if and only if its sum is not 0: the largest score's
+    // term is 1, and NaN is not 0 either)
+    // rows of this wave: query fragments, visible keys [lo, hi)
+    bf16x8 qf[NQ][T][W];
+    int64_t tok[NQ];
+    int lo[NQ], hi[NQ], head[NQ];
+    bool live[NQ];
+    int wlo = room, whi = 0;
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+      const int64_t r = tile * 16 * NQ + 16 * q + li;
+      live[q] = r < rows;
+      const int64_t rr = live[q] ? r : rows - 1;
+      const int i = (int)(rr / a.group);
+      head[q] = h * a.group + (int)(rr - (int64_t)i * a.group);
+      tok[q] = t0 + i;
+      const int pos = first + i;
+      hi[q] = a.causal ? min(len, max(pos + 1, 0)) : len;
+      lo[q] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      if (!live[q]) lo[q] = hi[q] = 0;
+      if (lo[q] < hi[q]) { wlo = min(wlo, lo[q]); whi = max(whi, hi[q]); }
+      const typename E::type* p = (const typename E::type*)a.q + tok[q] * a.qt + head[q] * a.qh;
+#pragma unroll
+      for (int n = 0; n < W; n++) {
+        float v[8];
+        bf16x8 f[T];
+        load8<E>(p + 8 * (W * kg + n), v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= sign;
+        split8<T>(v, f);
+#pragma unroll
+        for (int t = 0; t < T; t++) qf[q][t][n] = f[t];
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+      wlo = min(wlo, __shfl_xor(wlo, d));
+      whi = max(whi, __shfl_xor(whi, d));
+    }
+    const float c = fabsf(a.scale) * kLog2e;
+    const int klo = __builtin_amdgcn_readfirstlane(max(wlo & ~31, from));
+    const int khi = __builtin_amdgcn_readfirstlane(min(whi, to));
+
+    f32x4 o[NQ][2 * W] = {};
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; q++) { m[q] = -INFINITY; l[q] = 0.0f; }
+
+    const int step = WS == 4 ? 128 : 32;
+    for (int j0 = klo + (WS == 4 ? 32 * wave : 0); j0 < khi; j0 += step) {
+      // pages of the two halves; a page outside the pool holds no keys
+      const unsigned char *kc[2], *ks[2], *vc[2], *vs[2];
+      bool there[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int j = j0 + 16 * u;
+        int page = -1;
+        if (j < khi) page = __builtin_amdgcn_readfirstlane(table[j >> a.shift]);
+        there[u] = page >= 0 && page < a.n_pages;
+        const int64_t row = ((((int64_t)(there[u] ? page : 0) * a.heads + h) << a.shift) +
+                             (j & ((1 << a.shift) - 1)));
+        kc[u] = a.kc + row * (16 * W);
+        ks[u] = a.ks + row * W;
+        vc[u] = a.vc + row * (16 * W);
+        vs[u] = a.vs + row * W;
+      }
+      // keys
+      f32x4 s[2][NQ];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        unsigned kw[W];
+        __builtin_memcpy(kw, kc[u] + li * (16 * W) + kg * (4 * W), sizeof kw);
+        const int g0 = W * kg / 4, g1 = (W * kg + W - 1) / 4;
+        const float s0 = scale_of_byte(ks[u][li * W + g0]);
+        const float s1 = scale_of_byte(ks[u][li * W + g1]);
+#pragma unroll
+        for (int q = 0; q < NQ; q++) s[u][q] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < W; n++) {
+          const bf16x8 kf = fp4_word(kw[n], (W * kg + n) / 4 == g0 ? s0 : s1);
+#pragma unroll
+          for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int t = T - 1; t >= 0; t--) s[u][q] = mfma16(kf, qf[q][t][n], s[u][q]);
+        }
+      }
+      // masks, running maximum, exponentials
+      bf16x8 pf[NQ][PT];
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int j = j0 + 16 * u + 4 * kg + r;
+            const bool see = there[u] && j >= max(lo[q], from) && j < min(hi[q], to);
+            if (!see) s[u][q][r] = -INFINITY;
+            mx = fmaxf(mx, s[u][q][r]);
+          }
+        const float top = fmaxf(m[q], column_max(mx) * c);
+        const float sub = top == -INFINITY ? 0.0f : top;
+        const float keep = exp2_(m[q] - sub);
+        m[q] = top;
+        float p[8], sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          p[e] = exp2_(__builtin_fmaf(s[e / 4][q][e % 4], c, -sub));
+          sum += p[e];
+        }
+        l[q] = l[q] * keep + sum;
+#pragma unroll
+        for (int x = 0; x < 2 * W; x++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[q][x][r] *= keep;
+        split8<PT>(p, pf[q]);
+      }
+      // values: bytes W li .. + W - 1 of the lane's eight keys
+      unsigned vw[8][Lane<W>::vwords];
+      float vsc[8][2];
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int key = 4 * kg + e % 4;
+        const unsigned char* p = vc[e / 4] + key * (16 * W);
+        if constexpr (W == 1) {
+          vw[e][0] = p[li];
+        } else if constexpr (W == 2) {
+          vw[e][0] = *(const unsigned short*)(p + 2 * li);
+        } else if constexpr (W == 4 || W == 8) {
+          __builtin_memcpy(vw[e], p + W * li, W);
+        } else {
+          // W bytes by a word (two words) that stays inside the row
+          constexpr int span = W == 3 ? 4 : 8;
+          const int at = min(W * li, 16 * W - span), off = 8 * (W * li - at);
+          if constexpr (W == 3) {
+            unsigned t;
+            __builtin_memcpy(&t, p + at, 4);
+            vw[e][0] = t >> off;
+          } else {
+            unsigned long long t;
+            __builtin_memcpy(&t, p + at, 8);
+            t >>= off;
+            vw[e][0] = (unsigned)t;
+            vw[e][1] = (unsigned)(t >> 32);
+          }
+        }
+        const unsigned b0 = vs[e / 4][key * W + W * li / 16];
+        const unsigned b1 = Lane<W>::straddle ? vs[e / 4][key * W + (W * li + W - 1) / 16] : b0;
+        bad |= b0 == 255 || b1 == 255;
+        vsc[e][0] = scale_of_byte(b0);
+        vsc[e][1] = scale_of_byte(b1);
+      }
+      // A value block of NaN must not reach the rows that do not see its key
+      // (0 * NaN): its elements count as zero in the product, and the rows
+      // that do see it get their NaN from a product of ones.
+      if (__builtin_expect(__ballot(bad) != 0, 0)) {
+        bf16x8 ones[NQ];
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) ones[q][e] = s[e / 4][q][e % 4] == -INFINITY ? (__bf16)0.0f : (__bf16)1.0f;
+#pragma unroll
+        for (int x = 0; x < 2 * W; x++) {
+          bf16x8 nan;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const int half = Lane<W>::straddle && (W * li + x / 2) / 16 != W * li / 16;
+            nan[e] = vsc[e][half] == INFINITY ? (__bf16)1.0f : (__bf16)0.0f;
+          }
+#pragma unroll
+          for (int q = 0; q < NQ; q++) {
+            const f32x4 hit = mfma16(nan, ones[q], f32x4{0, 0, 0, 0});
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              if (hit[r] != 0.0f) o[q][x][r] = NAN;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+            if (vsc[e][i] == INFINITY) vsc[e][i] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < W; y++) {
+        unsigned pr[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const bool half = Lane<W>::straddle && (W * li + y) / 16 != W * li / 16;
+          const float sc = half ? vsc[e][1] : vsc[e][0];
+          const unsigned w = vw[e][y / 4];
+          pr[e] = y % 4 == 0 ? fp4_pair<0>(w, sc) : y % 4 == 1 ? fp4_pair<1>(w, sc)
+                : y % 4 == 2 ? fp4_pair<2>(w, sc) : fp4_pair<3>(w, sc);
+        }
+        u32x4 lo4, hi4;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          lo4[e] = __builtin_amdgcn_perm(pr[2 * e + 1], pr[2 * e], 0x05040100u);
+          hi4[e] = __builtin_amdgcn_perm(pr[2 * e + 1], pr[2 * e], 0x07060302u);
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+          for (int t = PT - 1; t >= 0; t--) {
+            o[q][2 * y] = mfma16(__builtin_bit_cast(bf16x8, lo4), pf[q][t], o[q][2 * y]);
+            o[q][2 * y + 1] = mfma16(__builtin_bit_cast(bf16x8, hi4), pf[q][t], o[q][2 * y + 1]);
+          }
+      }
+    }
+
+    // the sums of a row: over the lanes of its column, then (WS = 4) over the
+    // workgroup's waves, in their order
+#pragma unroll
+    for (int q = 0; q < NQ; q++) l[q] = column_sum(l[q]);
+    if constexpr (WS == 4) {
+      float* ml = lds;                          // [4][NQ * 16][2]
+      float* ol = lds + 4 * NQ * 32;            // [4 waves][NQ * 2W * 4][64]
+      __syncthreads();                          // (an earlier tile's reads)
+      if (kg == 0) {
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+          ml[((wave * NQ + q) * 16 + li) * 2] = m[q];
+          ml[((wave * NQ + q) * 16 + li) * 2 + 1] = l[q];
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < NQ; q++)
+#pragma unroll
+        for (int x = 0; x < 2 * W; x++)
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            ol[((wave * NQ + q) * 8 * W + r * 2 * W + x) * 64 + lane] = o[q][x][r];
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        float wm[4], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          wm[w] = ml[((w * NQ + q) * 16 + li) * 2];
+          top = fmaxf(top, wm[w]);
+        }
+        const float sub = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          wm[w] = exp2_(wm[w] - sub);
+          sum += wm[w] * ml[((w * NQ + q) * 16 + li) * 2 + 1];
+        }
+        m[q] = top;
+        l[q] = sum;
+        // wave r takes the rows d = 2 W (4 kg + r) + x of every lane group
+#pragma unroll
+        for (int x = 0; x < 2 * W; x++) {
+          float v = 0.0f;
+#pragma unroll
+          for (int w = 0; w < 4; w++)
+            v += wm[w] * ol[((w * NQ + q) * 8 * W + wave * 2 * W + x) * 64 + lane];
+          o[q][x][0] = v;
+        }
+      }
+    }
+    constexpr int NR = WS == 4 ? 1 : 4;
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+      if (!live[q]) continue;
+      const int64_t at = tok[q] * (a.heads * a.group) + head[q];
+      if (a.splits > 1) {
+        const int64_t part = (int64_t)split * a.tokens * (a.heads * a.group) + at;
+        if (kg == 0 && (WS == 1 || wave == 0)) {
+          a.part_ml[2 * part] = m[q];
+          a.part_ml[2 * part + 1] = l[q];
+        }
+        if (l[q] == 0.0f) continue;
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+          float* p = a.part_o + part * DH + 2 * W * (4 * kg + (WS == 4 ? wave : r));
+#pragma unroll
+          for (int x = 0; x < 2 * W; x++) p[x] = o[q][x][r];
+        }
+      } else {
+        const float inv = l[q] == 0.0f ? 0.0f : 1.0f / l[q];
+        if (a.lse && kg == 0 && (WS == 1 || wave == 0))
+          a.lse[at] = l[q] == 0.0f ? -INFINITY : m[q] * kLn2 + logf(l[q]);
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+          typename E::type* p = (typename E::type*)a.out + tok[q] * a.ot + head[q] * a.oh +
+                                2 * W * (4 * kg + (WS == 4 ? wave : r));
+          typename E::type t[2 * W];
+#pragma unroll
+          for (int x = 0; x < 2 * W; x++) t[x] = (typename E::type)(o[q][x][r] * inv);
+          __builtin_memcpy(p, t, sizeof t);
+        }
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: one wave a row, in the splits' order.
+template <typename E>
+__global__ __launch_bounds__(256) void attn4_join_kernel(Attn4 a, int dh) {
+  const int lane = threadIdx.x & 63;
+  const int qheads = a.heads * a.group;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), all = a.tokens * qheads;
+  if (row >= all) return;
+  const int64_t t = row / qheads;
+  if (a.starts && (t < a.starts[0] || t >= a.starts[a.batch])) return;
+  float m = -INFINITY, l = 0.0f;
+  if (lane < a.splits) {
+    m = a.part_ml[2 * (lane * all + row)];
+    l = a.part_ml[2 * (lane * all + row) + 1];
+  }
+  float top = m;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  const float w = exp2_(m - (top == -INFINITY ? 0.0f : top));
+  float sum = w * l;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  const unsigned long long some = __ballot(l != 0.0f);
+  typename E::type* out = (typename E::type*)a.out + t * a.ot + (row % qheads) * a.oh;
+  if (a.lse && lane == 0) a.lse[row] = some ? top * kLn2 + logf(sum) : -INFINITY;
+  const float inv = some ? 1.0f / sum : 0.0f;
+  for (int d = lane; d - lane < dh; d += 64) {
+    float v = 0.0f;
+    for (int s = 0; s < a.splits; s++) {
+      const float ws = __shfl(w, s);
+      if (some >> s & 1 && d < dh) v += ws * a.part_o[(s * all + row) * dh + d];
+    }
+    if (d < dh) out[d] = (typename E::type)(v * inv);
+  }
+}
+
+// ------------------------------------------------------------ host: the plan
+
+struct Attn4Plan {
+  int nq, ws;          // column tiles a wave; 4: the waves of a workgroup share their rows
+  int row_tiles;       // workgroups along the rows of a sequence and head
+  int splits;
+  int64_t chunk;
+  size_t workspace;
+};
+
+static Attn4Plan attn4_plan(const qph_cache4* c, const qph_attn4* p) {
+  Attn4Plan r{};
+  const int64_t rows = std::min<int64_t>((int64_t)p->max_new * (p->heads / c->heads), 1 << 30);
+  const int64_t keys = p->window > 0
+                           ? std::min<int64_t>(p->max_len, (int64_t)p->window + p->max_new + 31)
+                           : p->max_len;
+  const int64_t seqs = (int64_t)p->batch * c->heads;
+  const bool many = p->dtype != QPH_F32 ? c->dh <= 128 : c->dh <= 64;
+  if (rows <= 16) { r.nq = 1; r.ws = 4; }
+  else if (many && (rows + 63) / 64 * seqs >= 512) { r.nq = 2; r.ws = 1; }
+  else { r.nq = 1; r.ws = rows * seqs >= 64 * 512 ? 1 : 4; }
+  const int64_t tiles = (rows + 16 * r.nq - 1) / (16 * r.nq);
+  r.row_tiles = (int)std::min<int64_t>(std::max<int64_t>(1, r.ws == 4 ? tiles : (tiles + 3) / 4), 1 << 20);
+  r.splits = 1;
+  r.chunk = (int64_t)1 << 40;
+  const int64_t blocks = r.row_tiles * seqs;
+  if (r.ws == 4 && blocks < 2048 && keys > 512) {
+    int64_t n = std::min<int64_t>({(2048 + blocks - 1) / blocks, (keys + 255) / 256, 64});
+    r.chunk = ((keys + n - 1) / n + 127) / 128 * 128;
+    n = (keys + r.chunk - 1) / r.chunk;
+    if (n > 1) r.splits = (int)n;
+    else r.chunk = (int64_t)1 << 40;
+  }
+  if (r.splits > 1) r.workspace = (size_t)r.splits * p->tokens * p->heads * (c->dh + 2) * 4;
+  return r;
+}
+
+template <typename E, int W, int NQ, int WS>
+static int launch_attn4_one(const Attn4& a, hipStream_t s) {
+  const size_t lds = WS == 4 ? (size_t)4 * NQ * (32 + 2 * W * 4 * 64) * 4 : 0;
+  if (lds > 65536) QPH_TRY(allow_full_lds((const void*)attn4_kernel<E, W, NQ, WS>));
+  const int64_t blocks = (int64_t)a.row_tiles * a.splits * a.heads * a.batch;
+  hipLaunchKernelGGL((attn4_kernel<E, W, NQ, WS>), dim3((unsigned)blocks), dim3(256), lds, s, a);
+  return launch_check("attn4_kernel");
+}
+
+template <typename E, int W>
+static int launch_attn4_w(const Attn4& a, const Attn4Plan& p, hipStream_t s) {
+  if constexpr (W <= (E::terms == 3 ? 2 : 4)) {
+    if (p.nq == 2) return launch_attn4_one<E, W, 2, 1>(a, s);
+  }
+  if (p.ws == 1) return launch_attn4_one<E, W, 1, 1>(a, s);
+  return launch_attn4_one<E, W, 1, 4>(a, s);
+}
+
+template <typename E>
+static int launch_attn4(const Attn4& a, const Attn4Plan& p, int dh, hipStream_t s) {
+  switch (dh) {
+    case 32: QPH_TRY((launch_attn4_w<E, 1>(a, p, s))); break;
+    case 64: QPH_TRY((launch_attn4_w<E, 2>(a, p, s))); break;
+    case 96: QPH_TRY((launch_attn4_w<E, 3>(a, p, s))); break;
+    case 128: QPH_TRY((launch_attn4_w<E, 4>(a, p, s))); break;
+    case 192: QPH_TRY((launch_attn4_w<E, 6>(a, p, s))); break;
+    default: QPH_TRY((launch_attn4_w<E, 8>(a, p, s))); break;
+  }
+  if (a.splits == 1) return QPH_OK;
+  const int64_t rows = a.tokens * a.heads * a.group;
+  hipLaunchKernelGGL(attn4_join_kernel<E>, dim3(ceil_div(rows, 4)), dim3(256), 0, s, a, dh);
+  return launch_check("attn4_join_kernel");
+}
+
+static int attn4_check(const qph_cache4* c, const qph_attn4* p, int* shift) {
+  QPH_TRY(cache4_check(c, "attention_cache4", shift));
+  if (!p) return fail(QPH_EINVAL, "attention_cache4: NULL arguments");
+  if (!dtype_valid(p->dtype)) return fail(QPH_EINVAL, "attention_cache4: unknown element type");
+  if (p->tokens < 0 || p->batch < 0 || p->max_new < 0 || p->max_len < 0 || p->max_pages < 0 ||
+      p->window < 0)
+    return fail(QPH_EINVAL, "attention_cache4: negative size");
+  if (p->heads <= 0 || p->heads % c->heads)
+    return fail(QPH_EINVAL, "attention_cache4: query heads are no multiple of the cache's heads");
+  if (p->heads > 65536) return fail(QPH_EUNSUPPORTED, "attention_cache4: more than 65536 query heads");
+  if (!std::isfinite(p->scale) || p->scale == 0.0f)
+    return fail(QPH_EINVAL, "attention_cache4: scale is zero or not finite");
+  if (p->batch > INT32_MAX / c->heads || p->max_pages > INT32_MAX)
+    return fail(QPH_EUNSUPPORTED, "attention_cache4: more than 2^31 - 1 sequences' heads or pages");
+  if (!p->starts && p->batch && p->tokens != p->batch * (int64_t)p->max_new)
+    return fail(QPH_EINVAL, "attention_cache4: without starts, tokens must be batch * max_new");
+  if (p->tokens > ((int64_t)1 << 31) || (int64_t)p->tokens * p->heads > ((int64_t)1 << 33))
+    return fail(QPH_EUNSUPPORTED, "attention_cache4: too many rows for one call");
+  return QPH_OK;
+}
+
+}  // namespace qph
+
+using namespace qph;
+
+extern "C" {
+
+QPH_API int qph_attention_cache4_workspace(const qph_cache4* cache, const qph_attn4* args,
+                                           size_t* bytes) {
+  if (!bytes) return fail(QPH_EINVAL, "attention_cache4_workspace: NULL argument");
+  *bytes = 0;
+  int shift = 0;
+  QPH_TRY(attn4_check(cache, args, &shift));
+  if (args->tokens == 0 || args->batch == 0) return QPH_OK;
+  *bytes = attn4_plan(cache, args).workspace;
+  return QPH_OK;
+}
+
+QPH_API int qph_attention_cache4(qph_ctx* ctx, const qph_cache4* cache, const qph_attn4* args) {
+  int shift = 0;
+  QPH_TRY(attn4_check(cache, args, &shift));
+  const bool none = args->tokens == 0 || args->batch == 0;
+  if (!none && (!args->q || !args->out || !args->lens || (!args->page_table && args->max_pages)))
+    return fail(QPH_EINVAL, "attention_cache4: NULL argument");
+  const Attn4Plan p = none ? Attn4Plan{} : attn4_plan(cache, args);
+  if (p.workspace && (!args->workspace || args->workspace_bytes < p.workspace))
+    return fail(QPH_EINVAL, "attention_cache4: workspace of " + std::to_string(args->workspace_bytes) +
+                                " bytes, needs " + std::to_string(p.workspace));
+  if ((uintptr_t)args->workspace % 4)
+    return fail(QPH_EINVAL, "attention_cache4: workspace is not 4-byte aligned");
+  if ((int64_t)p.row_tiles * p.splits * cache->heads * args->batch > INT32_MAX)
+    return fail(QPH_EUNSUPPORTED, "attention_cache4: batch too large for one call");
+  if (!ctx) return fail(QPH_EINVAL, "null context");
+  if (none) return QPH_OK;
+  Attn4 a{};
+  a.kc = (const unsigned char*)cache->k_codes; a.ks = (const unsigned char*)cache->k_scales;
+  a.vc = (const unsigned char*)cache->v_codes; a.vs = (const unsigned char*)cache->v_scales;
+  a.n_pages = cache->n_pages;
+  a.shift = shift;
+  a.heads = cache->heads;
+  a.group = args->heads / cache->heads;
+  a.q = args->q; a.out = args->out; a.lse = args->lse;
+  a.qt = args->q_strides[0]; a.qh = args->q_strides[1];
+  a.ot = args->out_strides[0]; a.oh = args->out_strides[1];
+  a.tokens = args->tokens;
+  a.batch = (int)args->batch;
+  a.table = args->page_table;
+  a.table_stride = args->table_stride;
+  a.max_pages = (int)args->max_pages;
+  a.lens = args->lens;
+  a.starts = args->starts;
+  a.news = args->max_new;
+  a.scale = args->scale;
+  a.causal = args->causal != 0;
+  a.window = args->window;
+  a.row_tiles = p.row_tiles;
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  if (p.splits > 1) {
+    a.part_ml = (float*)args->workspace;
+    a.part_o = a.part_ml + (size_t)p.splits * args->tokens * args->heads * 2;
+  }
+  OnDevice dev(ctx);
+  QPH_TRY(dev.rc());
+  if (args->dtype == QPH_F32) return launch_attn4<F32>(a, p, cache->dh, ctx->stream);
+  if (args->dtype == QPH_F16) return launch_attn4<F16>(a, p, cache->dh, ctx->stream);
+  return launch_attn4<BF16>(a, p, cache->dh, ctx->stream);
+}
+
+}  // extern "C"

@@ -156,7 +156,7 @@ QPH_API int qph_ctx_set_stream(qph_ctx* ctx, void* stream) {
   CTX_CHECK(ctx);
   if (ctx->own_stream) QPH_TRY_HIP(hipStreamDestroy(ctx->stream));
   if (stream) {
-    ctx->stream = (hipStream_t)stream;
+    ctx->stream = stream == QPH_STREAM_DEFAULT ? nullptr : (hipStream_t)stream;
     ctx->own_stream = false;
   } else {
     QPH_TRY_HIP(hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking));

@@ -2,16 +2,21 @@
 (qppocr-kernels/src/lib.rs:28-40): conv2d / conv2d_res, convtranspose2d,
 sgemm / sgemm_res, matmul, softmax_last_dim, gelu_inplace, hardsigmoid,
 sigmoid_tensor, relu_inplace, reduce_mean (last axis), resize_nearest, and the
-CTC argmax of qppocr-core/src/pipeline/rec.rs.
+CTC argmax of qppocr-core/src/pipeline/rec.rs; and the 4-bit operators of a
+token-by-token decoder (quantize4, linear4, cache4_write, cache4_read,
+attention_cache4), which the reference lacks.
 
 Tensors are torch tensors on a ROCm device (torch is only the device-memory
 plumbing here); every call goes through the C ABI of libqppocr_hip.so.  Calls
 are synchronous with respect to torch's current stream: the stream is drained
 before the library's own stream runs the kernel, and the library stream is
-drained before returning.  Errors raise QphError (no silent fallback).
+drained before returning.  The 4-bit operators do not wait: they are enqueued on
+torch's current stream of the tensors' device, in its order, and may be captured
+into a graph.  Errors raise QphError (no silent fallback).
 """
 import ctypes
 import functools
+import threading
 
 import torch
 
@@ -452,3 +457,278 @@ def db_mask(pred, thresh, dilate=True):
         check(_lib.load().qph_db_mask(ctx, _ptr(pred), h, w, float(thresh), int(bool(dilate)),
                                       _ptr_any(out)))
     return out
+
+
+# ------------------------------------------- 4-bit weights and caches
+
+_DTYPES = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
+_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
+_queued = {}
+_queue_lock = threading.Lock()
+
+
+class _Queue:
+    """A library call on torch's current stream of a device, which does not wait.
+    The device's context for such calls takes the stream of each call under a
+    lock, since calls of several threads share it."""
+
+    __slots__ = ("device",)
+
+    def __init__(self, device):
+        self.device = device
+
+    def __enter__(self):
+        stream = torch.cuda.current_stream(self.device).cuda_stream or _lib.STREAM_DEFAULT
+        _queue_lock.acquire()
+        try:
+            entry = _queued.get(self.device)
+            if entry is None:
+                entry = _queued[self.device] = [new_context(self.device), None]
+            if entry[1] != stream:
+                check(_lib.load().qph_ctx_set_stream(entry[0], stream))
+                entry[1] = stream
+            return entry[0]
+        except BaseException:
+            _queue_lock.release()
+            raise
+
+    def __exit__(self, kind, value, trace):
+        _queue_lock.release()
+        return False
+
+
+def _dtype4(t, what):
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise ValueError(f"{what}: {t.dtype} is not float32, float16 or bfloat16")
+    return d
+
+
+def _on(what, device, **tensors):
+    """Refuses tensors (None: absent) that do not lie on the device."""
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
+
+
+def _plain(what, name, t, dtype, shape):
+    """Refuses a tensor that is not contiguous, of the dtype and of the shape."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of shape "
+                         f"{tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+
+
+class Weight4:
+    """A linear's weight [n, k] in 4 bits (the format: include/qppocr_hip.h):
+    codes uint8 [n, kp / 2] and scales uint8 [n, kp / 32], kp = k rounded up to
+    128, elements past k zero.  quantize4 makes one; a caller may bring the
+    two tensors."""
+
+    def __init__(self, codes, scales, k):
+        if codes.dim() != 2 or k <= 0:
+            raise ValueError("Weight4: codes [n, kp / 2] of k > 0 columns")
+        n, kp = codes.shape[0], (k + 127) // 128 * 128
+        _on("Weight4", codes.device, codes=codes, scales=scales)
+        _plain("Weight4", "codes", codes, torch.uint8, (n, kp // 2))
+        _plain("Weight4", "scales", scales, torch.uint8, (n, kp // 32))
+        if codes.data_ptr() % 16 or scales.data_ptr() % 4:
+            raise ValueError("Weight4: codes are not 16-byte or scales not 4-byte aligned")
+        self.codes, self.scales, self.n, self.k = codes, scales, n, int(k)
+
+
+def quantize4(w):
+    """The weight w [K, N] that linear takes (any strides; float32, float16 or
+    bfloat16) as a Weight4."""
+    if w.dim() != 2:
+        raise ValueError("quantize4: a weight [K, N]")
+    k, n = w.shape
+    if not k or not n:
+        raise ValueError("quantize4: empty weight")
+    d = _dtype4(w, "quantize4")
+    _on("quantize4", w.device, w=w)
+    kp = (k + 127) // 128 * 128
+    codes = torch.empty((n, kp // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((n, kp // 32), dtype=torch.uint8, device=w.device)
+    with _Queue(_dev(w)) as ctx:
+        check(_lib.load().qph_quantize4(ctx, w.data_ptr(), d, n, k, w.stride(1), w.stride(0),
+                                        codes.data_ptr(), scales.data_ptr()))
+    return Weight4(codes, scales, k)
+
+
+def linear4(x, w, bias=None, act_kind=ACT_NONE, residual=None):
+    """linear over a Weight4: act(x [..., K] . w + bias) + residual, in x's type
+    (float32, float16, bfloat16).  x's rows may lie apart (a slice of a packed
+    projection); bias and residual are contiguous and of x's type."""
+    d = _dtype4(x, "linear4")
+    if x.dim() < 1 or x.shape[-1] != w.k:
+        raise ValueError(f"linear4: x {tuple(x.shape)} against a weight of {w.k} inputs")
+    _on("linear4", w.codes.device, x=x, bias=bias, residual=residual)
+    shape = tuple(x.shape[:-1]) + (w.n,)
+    rows = x.numel() // w.k
+    x2 = x if x.dim() == 2 else x.reshape(rows, w.k)
+    if x2.stride(1) != 1 and w.k > 1:
+        x2 = x2.contiguous()
+    if bias is not None:
+        _plain("linear4", "bias", bias, x.dtype, (w.n,))
+    if residual is not None:
+        _plain("linear4", "residual", residual, x.dtype, shape)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    with _Queue(_dev(x)) as ctx:
+        check(_lib.load().qph_linear4(
+            ctx, x2.data_ptr(), d, x2.stride(0), w.codes.data_ptr(), w.scales.data_ptr(),
+            None if bias is None else bias.data_ptr(), rows, w.k, w.n, _act_ref(act_kind),
+            None if residual is None else residual.data_ptr(), y.data_ptr()))
+    return y
+
+
+class Cache4:
+    """A paged cache of keys and values in 4 bits (the format and layout:
+    include/qppocr_hip.h): codes uint8 [pages, heads, page size, dh / 2] and
+    scales uint8 [pages, heads, page size, dh / 32] of either.  cache4 makes
+    an empty one."""
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales):
+        if k_codes.dim() != 4:
+            raise ValueError("Cache4: codes [pages, heads, page size, dh / 2]")
+        pages, heads, page, half = k_codes.shape
+        _on("Cache4", k_codes.device, k_codes=k_codes, k_scales=k_scales, v_codes=v_codes,
+            v_scales=v_scales)
+        if 2 * half not in _HEAD_DIMS:
+            raise ValueError(f"Cache4: head dimension {2 * half} is not one of {_HEAD_DIMS}")
+        if page < 16 or page > 32768 or page & (page - 1):
+            raise ValueError(f"Cache4: page size {page} is no power of two from 16 to 32768")
+        if not pages or not heads:
+            raise ValueError("Cache4: empty cache")
+        for name, t, last in (("k_codes", k_codes, half), ("v_codes", v_codes, half),
+                              ("k_scales", k_scales, half // 16),
+                              ("v_scales", v_scales, half // 16)):
+            _plain("Cache4", name, t, torch.uint8, (pages, heads, page, last))
+        self.k_codes, self.k_scales = k_codes, k_scales
+        self.v_codes, self.v_scales = v_codes, v_scales
+        self.pages, self.heads, self.page_size, self.dh = pages, heads, page, 2 * half
+        self.device = k_codes.device
+        self._c = _lib.Cache4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                              v_scales.data_ptr(), pages, page, heads, 2 * half)
+        self._ref = ctypes.byref(self._c)
+
+
+def cache4(pages, page_size, heads, dh, device="cuda"):
+    """A Cache4 of zeros."""
+    if dh not in _HEAD_DIMS:
+        raise ValueError(f"cache4: head dimension {dh} is not one of {_HEAD_DIMS}")
+    def make(last, fill):
+        return torch.full((pages, heads, page_size, last), fill, dtype=torch.uint8, device=device)
+    return Cache4(make(dh // 2, 0), make(dh // 32, 27), make(dh // 2, 0), make(dh // 32, 27))
+
+
+def _rows4(what, name, t, cache, tokens, heads):
+    if tuple(t.shape) != (tokens, heads, cache.dh) or (t.stride(2) != 1 and t.numel()):
+        raise ValueError(f"{what}: {name} must be [{tokens}, {heads}, {cache.dh}] with neighbouring "
+                         f"elements of a head, not {tuple(t.shape)} of strides {t.stride()}")
+    return (_lib.I64 * 2)(t.stride(0), t.stride(1))
+
+
+def cache4_write(cache, k, v, slots):
+    """Quantises tokens' keys and values [tokens, heads, dh] (tokens and heads
+    of any strides) into their slots, int64 [tokens]: page * page_size + place.
+    A slot outside the pool (-1 for a padded token) is skipped; the others must
+    differ."""
+    d = _dtype4(k, "cache4_write")
+    if k.dim() != 3 or v.dtype != k.dtype:
+        raise ValueError("cache4_write: k and v [tokens, heads, dh] of one type")
+    n = k.shape[0]
+    _on("cache4_write", cache.device, k=k, v=v, slots=slots)
+    ks = _rows4("cache4_write", "k", k, cache, n, cache.heads)
+    vs = _rows4("cache4_write", "v", v, cache, n, cache.heads)
+    _plain("cache4_write", "slots", slots, torch.int64, (n,))
+    with _Queue(_dev(k)) as ctx:
+        check(_lib.load().qph_cache4_write(ctx, cache._ref, k.data_ptr(), v.data_ptr(), d, n, ks,
+                                           vs, slots.data_ptr()))
+
+
+def cache4_read(cache, slots, dtype=torch.float32, out=None):
+    """The tokens of slots, int64 [tokens], as (k, v) [tokens, heads, dh] of
+    dtype; zeros for a slot outside the pool.  out: such a pair to write into
+    (tokens and heads of any strides)."""
+    if slots.dim() != 1:
+        raise ValueError("cache4_read: slots [tokens]")
+    n = slots.shape[0]
+    if out is None:
+        shape = (n, cache.heads, cache.dh)
+        out = (torch.empty(shape, dtype=dtype, device=cache.device),
+               torch.empty(shape, dtype=dtype, device=cache.device))
+    k, v = out
+    d = _dtype4(k, "cache4_read")
+    if v.dtype != k.dtype:
+        raise ValueError("cache4_read: k and v of one type")
+    _on("cache4_read", cache.device, k=k, v=v, slots=slots)
+    ks = _rows4("cache4_read", "k", k, cache, n, cache.heads)
+    vs = _rows4("cache4_read", "v", v, cache, n, cache.heads)
+    _plain("cache4_read", "slots", slots, torch.int64, (n,))
+    with _Queue(_dev(slots)) as ctx:
+        check(_lib.load().qph_cache4_read(ctx, cache._ref, k.data_ptr(), v.data_ptr(), d, n, ks,
+                                          vs, slots.data_ptr()))
+    return k, v
+
+
+def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=None, max_len=None,
+                     causal=True, window=0, lse=False, out=None):
+    """Attention of new tokens q [tokens, heads, dh] over a Cache4 that holds
+    their keys and values already.
+
+    page_table int32 [batch, pages] and lens int32 [batch] name each sequence's
+    pages and cached tokens, its new ones the last of them.  starts int32
+    [batch + 1]: sequence b's new tokens are q[starts[b]:starts[b + 1]], at most
+    max_new (needed then); without starts every sequence has tokens / batch.
+    max_len bounds lens (default: all of the table's pages).  causal hides
+    later keys, window > 0 all but the last `window` up to a token's own.  A
+    row that sees no key is zero; rows of no sequence keep what out holds.
+    Returns out, or (out, lse) with the sums' logarithms, float32 [tokens,
+    heads] (-infinity where no key is seen; a new tensor's rows of no sequence
+    are undefined)."""
+    what = "attention_cache4"
+    d = _dtype4(q, what)
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q [tokens, heads, dh]")
+    tokens, heads = q.shape[0], q.shape[1]
+    _on(what, cache.device, q=q, page_table=page_table, lens=lens, starts=starts, out=out)
+    qs = _rows4(what, "q", q, cache, tokens, heads)
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (
+            page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise ValueError(f"{what}: page_table int32 [batch, pages], rows contiguous")
+    batch, pages = page_table.shape
+    _plain(what, "lens", lens, torch.int32, (batch,))
+    if starts is not None:
+        _plain(what, "starts", starts, torch.int32, (batch + 1,))
+        if max_new is None:
+            raise ValueError(f"{what}: starts need max_new")
+    elif batch and tokens % batch:
+        raise ValueError(f"{what}: {tokens} tokens for {batch} sequences need starts")
+    elif batch:
+        if max_new is not None and max_new != tokens // batch:
+            raise ValueError(f"{what}: max_new {max_new} without starts, where every sequence "
+                             f"has {tokens // batch}")
+        max_new = tokens // batch
+    else:
+        max_new = 0
+    if max_len is None:
+        max_len = min(pages * cache.page_size, 0x7fffff00)
+    if out is None:
+        out = torch.empty((tokens, heads, cache.dh), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype:
+        raise ValueError(f"{what}: out is {out.dtype}, q {q.dtype}")
+    os = _rows4(what, "out", out, cache, tokens, heads)
+    sums = torch.empty((tokens, heads), device=q.device) if lse else None
+    a = _lib.Attn4(q.data_ptr(), out.data_ptr(), None if sums is None else sums.data_ptr(), qs, os,
+                   tokens, batch, page_table.data_ptr(), page_table.stride(0), pages,
+                   lens.data_ptr(), None if starts is None else starts.data_ptr(), d, heads,
+                   int(max_new), int(max_len), float(scale), int(bool(causal)), int(window), None,
+                   0)
+    lib, ref, size = _lib.load(), ctypes.byref(a), ctypes.c_size_t()
+    check(lib.qph_attention_cache4_workspace(cache._ref, ref, ctypes.byref(size)))
+    if size.value:
+        work = torch.empty(size.value, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), size.value
+    with _Queue(_dev(q)) as ctx:
+        check(lib.qph_attention_cache4(ctx, cache._ref, ref))
+    return (out, sums) if lse else out
