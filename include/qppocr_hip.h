@@ -394,7 +394,7 @@ QPH_API int qph_cache4_read(qph_ctx* ctx, const qph_cache4* cache, void* k, void
  * bits (24 for float32) in the second product.
  * page_table, lens and starts are device memory.  The workspace (device, of
  * qph_attention_cache4_workspace bytes for the same arguments, which depend on
- * no device data) is this call's until it has run; calls that may overlap need
+ * no device data; 16-byte aligned) is this call's until it has run; calls that may overlap need
  * one each. */
 typedef struct {
   const void* q;              /* [tokens][heads][dh], strides {token, head} */

@@ -34,6 +34,11 @@ CFLAGS = [
     "-Wno-unused-function",
 ]
 
+# The accumulators of the 4-bit kernels are also read and scaled by VALU
+# instructions, which cannot reach the accumulation registers: without this the
+# compiler copies them there and back in every step.
+EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm",
+             "-amdgpu-kernarg-preload-count=16"] for f in ("qph_fp4.hip", "qph_attn4.hip")}
 
 # host-code sanitizers only (the device code is built as usual): each
 # -fsanitize= goes to the host compilation alone
@@ -44,7 +49,7 @@ SANITIZE = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=unde
 
 def _compile(src, build_dir=None, extra=()):
     obj = os.path.join(build_dir or BUILD, os.path.splitext(src)[0] + ".o")
-    cmd = [HIPCC] + CFLAGS + list(extra) + ["-c", os.path.join(CSRC, src), "-o", obj]
+    cmd = [HIPCC] + CFLAGS + EXTRA.get(src, []) + list(extra) + ["-c", os.path.join(CSRC, src), "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     err = "\n".join(l for l in r.stderr.splitlines() if "packed-fp32-ops" not in l)
     if r.returncode != 0:

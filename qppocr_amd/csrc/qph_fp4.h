@@ -94,8 +94,8 @@ __device__ __forceinline__ void store8(typename E::type* p, const float v[8]) {
 // Eight float32 as T bfloat16 terms that sum to them: each but the last cut
 // off (so that no term overflows, and the rest is exact), the last rounded to
 // nearest (exact too where the terms hold all bits).  An infinity is its own
-// first term and leaves nothing; a NaN stays one.
-template <int T>
+// first term and leaves nothing (INF false: there are none); a NaN stays one.
+template <int T, bool INF = true>
 __device__ __forceinline__ void split8(const float v[8], bf16x8 out[T]) {
   float r[8];
 #pragma unroll
@@ -115,7 +115,7 @@ __device__ __forceinline__ void split8(const float v[8], bf16x8 out[T]) {
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const float c = __uint_as_float(__float_as_uint(r[i]) & 0xffff0000u);
-        r[i] = r[i] == c ? 0.0f : r[i] - c;
+        r[i] = INF && r[i] == c ? 0.0f : r[i] - c;
       }
     }
   }
