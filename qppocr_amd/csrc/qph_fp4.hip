@@ -145,100 +145,448 @@ __device__ __forceinline__ float act4_apply(float v, const Act& a) {
   return act_apply(v, a);
 }
 
-// y[r][j] = act(sum_k x[r][k] W[j][k] + bias[j]) + res[r][j].  A wave takes
-// 16 NT columns j (MFMA rows) and 16 NQ rows r (MFMA columns); the waves of a
-// workgroup take the chunks of k in turn and their sums are added in LDS in
-// the waves' order.  A lane holds 32 neighbouring k of one column, one block:
-// 16 bytes of codes and one scale.
-template <typename E, int NQ, int NT>
-__global__ __launch_bounds__(1024) void linear4_kernel(Lin4 a) {
-  constexpr int T = E::terms;
-  extern __shared__ float red[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int li = lane & 15, kg = lane >> 4;
-  const int64_t j0 = (int64_t)blockIdx.x * (16 * NT), r0 = (int64_t)blockIdx.y * (16 * NQ);
-  const unsigned char* wc[NT];
-  const unsigned char* wsc[NT];
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <int B>
+__device__ __forceinline__ unsigned fp4_pair_f16(unsigned w, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, B));
+}
+
+__device__ __forceinline__ f16x8 fp4_word_f16(unsigned w, float scale) {
+  const u32x4 v = {fp4_pair_f16<0>(w, scale), fp4_pair_f16<1>(w, scale), fp4_pair_f16<2>(w, scale),
+                   fp4_pair_f16<3>(w, scale)};
+  return __builtin_bit_cast(f16x8, v);
+}
+
+// A block whose numbers are exact in float16: scale bytes 104 to 140 (6 2^13
+// to half of 2^-23), or all codes zero.
+__device__ __forceinline__ bool fits_f16(unsigned s, u32x4 w) {
+  return s - 104u <= 36u || (s < 104u && ((w[0] | w[1] | w[2] | w[3]) & 0x77777777u) == 0);
+}
+
+// y[r][j] = act(sum_k x[r][k] W[j][k] + bias[j]) + res[r][j], on MFMAs whose
+// rows are 16 columns j and whose columns are 16 rows r.  A lane holds 32
+// neighbouring k of one column, one block: 16 bytes of codes and one scale, so
+// it needs the 32 neighbouring elements of a row of x beside them.  x comes in
+// whole lines and is turned in LDS; straight from memory each load would touch
+// 64 lines (32 rows of 4096 x 12288: 41 us so, 24 through LDS).  float16 x
+// against weights that are exact in float16 (any of ordinary size) is one
+// float16 product of full precision, otherwise x is split into bfloat16 terms.
+
+// 16 bytes of a row of x from element k of it on; past the end of the row zeros.
+template <typename E>
+__device__ __forceinline__ u32x4 x_piece(const typename E::type* row, int64_t k, int64_t end) {
+  constexpr int elems = 16 / sizeof(typename E::type);
+  u32x4 v = {0, 0, 0, 0};
+  if (k + elems <= end) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else if (k < end) {
+    typename E::type t[elems];
 #pragma unroll
-  for (int t = 0; t < NT; t++) {
-    const int64_t j = min(j0 + 16 * t + li, a.n - 1);
-    wc[t] = a.codes + j * a.chunks * 64 + kg * 16;
-    wsc[t] = a.scales + j * a.chunks * 4 + kg;
+    for (int i = 0; i < elems; i++) t[i] = k + i < end ? row[k + i] : (typename E::type)0.0f;
+    __builtin_memcpy(&v, t, 16);
   }
-  const typename E::type* xr[NQ];
+  return v;
+}
+
+// The lane's scale out of its column's four, into the exponent's place: the
+// conversions read nothing else of that operand.
+__device__ __forceinline__ float lane_scale(unsigned four, int kg) {
+  return __uint_as_float(__builtin_amdgcn_alignbit(four, four, (8 * kg + 9) & 31));
+}
+
+// The products of a chunk: w and four a lane's 32 codes and its column's four
+// scales for each of NT column tiles, part(m, xf) the lane's 32 elements of x,
+// eight at a time, for each of NQ row tiles.  TS terms: the bfloat16 terms, or
+// with float16 the elements themselves.
+template <typename E, int NQ, int NT, int TS, typename Part>
+__device__ __forceinline__ void chunk_products(const u32x4* w, const unsigned* four, int kg,
+                                               Part part, f32x4 (&acc)[NT][NQ]) {
+  float sc[NT];
 #pragma unroll
-  for (int q = 0; q < NQ; q++)
-    xr[q] = (const typename E::type*)a.x + min(r0 + 16 * q + li, a.rows - 1) * a.xs;
-  f32x4 acc[NT][NQ] = {};
-  for (int64_t c = wave; c < a.chunks; c += waves) {
-    u32x4 w[NT];
-    float sc[NT];
+  for (int i = 0; i < NT; i++) sc[i] = lane_scale(four[i], kg);
+  bool f16 = false;
+  if constexpr (E::terms == 2) {
+    bool fits = true;
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      w[t] = *(const u32x4*)(wc[t] + c * 64);
-      sc[t] = scale_of_byte(wsc[t][c * 4]);
-    }
-    const int64_t k0 = c * 128 + kg * 32;
-    const bool whole = c * 128 + 128 <= a.k;
+    for (int i = 0; i < NT; i++) fits &= fits_f16(four[i] >> (8 * kg) & 255, w[i]);
+    f16 = __all(fits);
+  }
+  if (E::terms == 2 && f16) {
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-      bf16x8 xf[NQ][T];
+    for (int m = 0; m < 4; m++) {
+      u32x4 x[NQ][TS];
+      part(m, x);
 #pragma unroll
-      for (int q = 0; q < NQ; q++) {
-        float v[8];
-        if (whole) load8<E>(xr[q] + k0 + 8 * n, v);
-        else load8_upto<E>(xr[q] + k0 + 8 * n, (int)max((int64_t)0, min((int64_t)8, a.k - k0 - 8 * n)), v);
-        split8<T>(v, xf[q]);
-      }
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        const bf16x8 wf = fp4_word(w[t][n], sc[t]);
+      for (int i = 0; i < NT; i++) {
+        const f16x8 wf = fp4_word_f16(w[i][m], sc[i]);
 #pragma unroll
         for (int q = 0; q < NQ; q++)
-#pragma unroll
-          for (int s = T - 1; s >= 0; s--) acc[t][q] = mfma16(wf, xf[q][s], acc[t][q]);
+          acc[i][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(f16x8, x[q][0]),
+                                                             acc[i][q], 0, 0, 0);
       }
     }
-  }
-  // sums of the waves, in their order
+  } else {
 #pragma unroll
-  for (int t = 0; t < NT; t++)
+    for (int m = 0; m < 4; m++) {
+      u32x4 x[NQ][TS];
+      bf16x8 xf[NQ][E::terms];
+      part(m, x);
 #pragma unroll
-    for (int q = 0; q < NQ; q++)
+      for (int q = 0; q < NQ; q++) {
+        if constexpr (E::terms == 2) {
+          const f16x8 h = __builtin_bit_cast(f16x8, x[q][0]);
+          float v[8];
 #pragma unroll
-      for (int r = 0; r < 4; r++)
-        red[(((wave * NQ + q) * 16 + li) * NT + t) * 16 + 4 * kg + r] = acc[t][q][r];
-  __syncthreads();
-  constexpr int tile = NQ * 16 * NT * 16;
-  for (int i = threadIdx.x; i < tile; i += blockDim.x) {
-    const int64_t r = r0 + i / (16 * NT), j = j0 + i % (16 * NT);
-    if (r >= a.rows || j >= a.n) continue;
-    float v = 0.0f;
-    for (int w = 0; w < waves; w++) v += red[w * tile + i];
-    if (a.bias) v += (float)((const typename E::type*)a.bias)[j];
-    v = act4_apply(v, a.act);
-    if (a.res) v += (float)((const typename E::type*)a.res)[r * a.n + j];
-    ((typename E::type*)a.y)[r * a.n + j] = (typename E::type)v;
+          for (int e = 0; e < 8; e++) v[e] = (float)h[e];
+          split8<2>(v, xf[q]);
+        } else {
+#pragma unroll
+          for (int t = 0; t < TS; t++) xf[q][t] = __builtin_bit_cast(bf16x8, x[q][t]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT; i++) {
+        const bf16x8 wf = fp4_word(w[i][m], sc[i]);
+#pragma unroll
+        for (int t = E::terms - 1; t >= 0; t--)
+#pragma unroll
+          for (int q = 0; q < NQ; q++) acc[i][q] = mfma16(wf, xf[q][t], acc[i][q]);
+      }
+    }
   }
 }
 
-template <typename E, int NQ, int NT>
-static int launch_linear4_tile(const Lin4& a, hipStream_t s) {
-  // waves along k: a workgroup of up to 8, each with a chunk at least, and no
-  // more than 64 KB of sums
-  const int tile = NQ * 16 * NT * 16 * 4;
+// Four neighbouring columns' results.
+template <typename E>
+__device__ __forceinline__ void linear4_store(const Lin4& a, int64_t r, int64_t j, f32x4 v) {
+  typedef typename E::type T;
+  if (r >= a.rows || j >= a.n) return;
+  const T* bias = (const T*)a.bias + j;
+  const T* res = (const T*)a.res + (r * a.n + j);
+  T* y = (T*)a.y + (r * a.n + j);
+  const bool whole = j + 4 <= a.n;
+  T b[4] = {}, s[4] = {}, o[4];
+  if (whole) {
+    if (a.bias) __builtin_memcpy(b, bias, sizeof b);
+    if (a.res) __builtin_memcpy(s, res, sizeof s);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (a.bias && j + e < a.n) b[e] = bias[e];
+      if (a.res && j + e < a.n) s[e] = res[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (a.bias) v[e] += (float)b[e];
+    if (a.act.kind) v[e] = act4_apply(v[e], a.act);
+    if (a.res) v[e] += (float)s[e];
+    o[e] = (T)v[e];
+  }
+  if (whole) {
+    __builtin_memcpy(y, o, sizeof o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (j + e < a.n) y[e] = o[e];
+  }
+}
+
+// Few rows: bound by the weights' way from memory, each read once, and by the
+// latencies before and after it, so everything is asked for at once.  The waves
+// of a workgroup share 16 NT columns and take groups of U chunks of 128 k in
+// turn: the group's x, then the codes and scales of all NT column tiles.  The
+// waves' sums are added in LDS in their order.  The arguments that the loads
+// need come first: they are in registers when the wave starts.
+template <typename E, int NQ, int NT, int U>
+__global__ __launch_bounds__(512) void linear4_few_kernel(const typename E::type* x,
+                                                          const unsigned char* codes,
+                                                          const unsigned char* scales, int64_t xs,
+                                                          int rows, int k, int n, int chunks,
+                                                          Lin4 a) {
+  constexpr int size = sizeof(typename E::type);
+  constexpr int TS = E::terms == 3 ? 3 : 1;
+  constexpr int pieces = 8 * size, per = 2 * size;   // 16-byte pieces of 128 k; loads for 16 rows
+  constexpr int elems = 16 / size, step = 64 / pieces;
+  extern __shared__ __align__(16) char lds4[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = blockDim.x >> 6;
+  const int li = lane & 15, kg = lane >> 4;
+  const int j0 = blockIdx.x * (16 * NT), r0 = blockIdx.y * (16 * NQ);
+  char* part = lds4 + wave * (NQ * per * 1024);
+  f32x4 acc[NT][NQ] = {};
+  for (int c0 = wave * U; c0 < chunks; c0 += waves * U) {
+    // x: piece lane % pieces of rows lane / pieces + step i
+    u32x4 xv[U][NQ][per];
+    const bool inside = (c0 + U) * 128 <= k;
+#pragma unroll
+    for (int q = 0; q < NQ; q++)
+#pragma unroll
+      for (int i = 0; i < per; i++) {
+        if (r0 + 16 * q + step * i >= rows) continue;     // (the columns of no row hold anything)
+        const int r = min(r0 + 16 * q + step * i + lane / pieces, rows - 1);
+        const int at = c0 * 128 + (lane % pieces) * elems;
+        const typename E::type* row = x + r * xs;
+        if (inside) {
+#pragma unroll
+          for (int u = 0; u < U; u++) __builtin_memcpy(&xv[u][q][i], row + at + u * 128, 16);
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; u++) xv[u][q][i] = x_piece<E>(row, at + u * 128, k);
+        }
+      }
+    // (a group that ends past the last chunk: that chunk again, against zeros)
+    u32x4 w[NT][U];
+    unsigned four[NT][U];
+    const bool full = c0 + U <= chunks;
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+      const int64_t at = (int64_t)min(j0 + 16 * i + li, n - 1) * chunks + c0;
+      const unsigned char* cp = codes + at * 64 + kg * 16;
+      const unsigned char* sp = scales + at * 4;
+      if (full) {
+#pragma unroll
+        for (int u = 0; u < U; u++) w[i][u] = *(const u32x4*)(cp + u * 64);
+        __builtin_memcpy(four[i], sp, 4 * U);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const int c = min(u, chunks - 1 - c0);
+          w[i][u] = *(const u32x4*)(cp + c * 64);
+          four[i][u] = *(const unsigned*)(sp + c * 4);
+        }
+      }
+    }
+    // piece p of row r at place p ^ r of the row: neither the rows' stores nor
+    // the columns' loads meet in a bank
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+      for (int q = 0; q < NQ; q++)
+#pragma unroll
+        for (int i = 0; i < per; i++) {
+          if (r0 + 16 * q + step * i >= rows) continue;
+          const int r = step * i + lane / pieces;
+          *(u32x4*)(part + ((q * 16 + r) * pieces + ((lane % pieces) ^ r)) * 16) = xv[u][q][i];
+        }
+      u32x4 wu[NT];
+      unsigned fu[NT];
+#pragma unroll
+      for (int i = 0; i < NT; i++) { wu[i] = w[i][u]; fu[i] = four[i][u]; }
+      chunk_products<E, NQ, NT, TS>(wu, fu, kg, [&](int m, u32x4 (&xf)[NQ][TS]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+          const char* row = part + (q * 16 + li) * pieces * 16;
+          const int p = (4 * kg + m) * (size / 2);
+          const u32x4 v0 = *(const u32x4*)(row + (p ^ li) * 16);
+          if constexpr (E::terms == 3) {
+            const u32x4 v1 = *(const u32x4*)(row + ((p + 1) ^ li) * 16);
+            float v[8];
+            bf16x8 t[3];
+            __builtin_memcpy(v, &v0, 16);
+            __builtin_memcpy(v + 4, &v1, 16);
+            split8<3>(v, t);
+#pragma unroll
+            for (int i = 0; i < 3; i++) xf[q][i] = __builtin_bit_cast(u32x4, t[i]);
+          } else {
+            xf[q][0] = v0;
+          }
+        }
+      }, acc);
+    }
+  }
+  float* red = (float*)lds4;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NT; i++)
+#pragma unroll
+    for (int q = 0; q < NQ; q++)
+      *(f32x4*)&red[(((wave * NQ + q) * 16 + li) * NT + i) * 16 + 4 * kg] = acc[i][q];
+  __syncthreads();
+  constexpr int tile = NQ * 16 * NT * 16;
+  for (int i = 4 * threadIdx.x; i < tile; i += 4 * blockDim.x) {
+    f32x4 v = *(const f32x4*)&red[i];
+    for (int w = 1; w < waves; w++) v += *(const f32x4*)&red[w * tile + i];
+    linear4_store<E>(a, r0 + i / (16 * NT), j0 + i % (16 * NT), v);
+  }
+}
+
+// More rows: a workgroup takes 16 NQ rows and 64 NT columns, its waves 16 NT
+// columns of one half of every 256 k.  x is staged in LDS for all of them,
+// split into its terms once, in the order of the MFMA's operand; two buffers,
+// and the loads of the next D parts in flight.
+template <typename E, int NQ, int NT, int D>
+__global__ __launch_bounds__(512) void linear4_rows_kernel(const typename E::type* x,
+                                                           const unsigned char* codes,
+                                                           const unsigned char* scales, int64_t xs,
+                                                           int rows, int k, int n, int chunks,
+                                                           Lin4 a) {
+  typedef typename E::type T;
+  constexpr int TS = E::terms == 3 ? 3 : 1;
+  constexpr int half = 4 * NQ * TS * 1024, buffer = 2 * half;
+  extern __shared__ __align__(16) char lds4[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave & 3, wk = wave >> 2;
+  const int li = lane & 15, kg = lane >> 4;
+  const int j0 = blockIdx.x * (64 * NT), r0 = blockIdx.y * (16 * NQ);
+  const unsigned char *cp[NT], *sp[NT];
+#pragma unroll
+  for (int i = 0; i < NT; i++) {
+    const int64_t at = (int64_t)min(j0 + 16 * (wn * NT + i) + li, n - 1) * chunks;
+    cp[i] = codes + at * 64 + kg * 16;
+    sp[i] = scales + at * 4;
+  }
+  // staged by this thread: eight elements, part p of 32, of row tid / 32 of each tile
+  const int p = tid & 31, row = tid >> 5, ph = p >> 4, pk = p >> 2 & 3, pn = p & 3;
+  const T* xr[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; q++) xr[q] = x + min(r0 + 16 * q + row, rows - 1) * xs;
+  char* put = lds4 + ph * half + (pk * 16 + (row ^ (4 * pk + pn))) * 16;
+
+  constexpr int XV = sizeof(T) / 2;     // 16-byte loads of eight elements
+  struct Part {
+    u32x4 x[NQ][XV], w[NT];
+    unsigned four[NT];
+  };
+  const int parts = (chunks + 1) / 2;
+  auto load = [&](int it, Part& s) __attribute__((always_inline)) {
+    if (it >= parts) return;
+    const int at = it * 256 + p * 8;
+#pragma unroll
+    for (int q = 0; q < NQ; q++)
+#pragma unroll
+      for (int i = 0; i < XV; i++) {
+        if (it * 256 + 256 <= k) __builtin_memcpy(&s.x[q][i], xr[q] + at + i * (8 / XV), 16);
+        else s.x[q][i] = x_piece<E>(xr[q], at + i * (8 / XV), k);
+      }
+    const int c = min(2 * it + wk, chunks - 1);     // (past the last: against zeros)
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+      s.w[i] = *(const u32x4*)(cp[i] + (int64_t)c * 64);
+      s.four[i] = *(const unsigned*)(sp[i] + (int64_t)c * 4);
+    }
+  };
+  auto stage = [&](const Part& s, int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+      if constexpr (TS == 3) {
+        float v[8];
+        bf16x8 t[3];
+        __builtin_memcpy(v, &s.x[q][0], 32);
+        split8<3>(v, t);
+#pragma unroll
+        for (int i = 0; i < 3; i++) *(bf16x8*)(put + b * buffer + ((pn * NQ + q) * 3 + i) * 1024) = t[i];
+      } else {
+        *(u32x4*)(put + b * buffer + (pn * NQ + q) * 1024) = s.x[q][0];
+      }
+    }
+  };
+  f32x4 acc[NT][NQ] = {};
+  auto compute = [&](const Part& s, int b) __attribute__((always_inline)) {
+    const char* from = lds4 + b * buffer + wk * half;
+    chunk_products<E, NQ, NT, TS>(s.w, s.four, kg, [&](int m, u32x4 (&xf)[NQ][TS]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int q = 0; q < NQ; q++)
+#pragma unroll
+        for (int t = 0; t < TS; t++)
+          xf[q][t] = *(const u32x4*)(from + ((m * NQ + q) * TS + t) * 1024 +
+                                     (kg * 16 + (li ^ (4 * kg + m))) * 16);
+    }, acc);
+  };
+  // D is even, so that part it is in buffer it % 2: the one that a part is
+  // staged into was read before the barrier that the part before it passed
+  static_assert(D % 2 == 0, "two buffers");
+  Part s[D];
+#pragma unroll
+  for (int d = 0; d < D; d++) load(d, s[d]);
+  for (int it = 0; it < parts; it += D) {
+#pragma unroll
+    for (int d = 0; d < D; d++) {
+      if (it + d >= parts) break;
+      stage(s[d], d & 1);
+      __syncthreads();
+      compute(s[d], d & 1);
+      load(it + d + D, s[d]);
+    }
+  }
+  // the two halves' sums
+  float* red = (float*)lds4;
+  __syncthreads();
+  constexpr int cols = 64 * NT, tile = 16 * NQ * cols;
+#pragma unroll
+  for (int i = 0; i < NT; i++)
+#pragma unroll
+    for (int q = 0; q < NQ; q++)
+      *(f32x4*)&red[wk * tile + (q * 16 + li) * cols + (wn * NT + i) * 16 + 4 * kg] = acc[i][q];
+  __syncthreads();
+  for (int i = 4 * tid; i < tile; i += 2048)
+    linear4_store<E>(a, r0 + i / cols, j0 + i % cols, *(f32x4*)&red[i] + *(f32x4*)&red[tile + i]);
+}
+
+template <typename E, int NQ, int NT, int U>
+static int launch_linear4_few(const Lin4& a, hipStream_t s) {
+  // up to 8 waves along k, with a group of chunks each
+  const int part = std::max(NQ * 16 * NT * 16 * 4, NQ * 2 * (int)sizeof(typename E::type) * 1024);
   int waves = 8;
-  while (waves > 1 && (waves > a.chunks || waves * tile > 65536)) waves /= 2;
+  while (waves > 1 && (waves / 2) * U >= a.chunks) waves /= 2;
+  if (waves * part > 65536) QPH_TRY(allow_full_lds((const void*)linear4_few_kernel<E, NQ, NT, U>));
   const dim3 grid(ceil_div(a.n, 16 * NT), ceil_div(a.rows, 16 * NQ));
-  hipLaunchKernelGGL((linear4_kernel<E, NQ, NT>), grid, dim3(64 * waves), waves * tile, s, a);
-  return launch_check("linear4_kernel");
+  hipLaunchKernelGGL((linear4_few_kernel<E, NQ, NT, U>), grid, dim3(64 * waves), waves * part, s,
+                     (const typename E::type*)a.x, a.codes, a.scales, a.xs, (int)a.rows, (int)a.k,
+                     (int)a.n, (int)a.chunks, a);
+  return launch_check("linear4_few_kernel");
+}
+
+template <typename E, int NQ, int NT, int D>
+static int launch_linear4_rows(const Lin4& a, hipStream_t s) {
+  constexpr int TS = E::terms == 3 ? 3 : 1;
+  const int lds = std::max(4 * 4 * NQ * TS * 1024, 2 * 16 * NQ * 64 * NT * 4);
+  if (lds > 65536) QPH_TRY(allow_full_lds((const void*)linear4_rows_kernel<E, NQ, NT, D>));
+  const dim3 grid(ceil_div(a.n, 64 * NT), ceil_div(a.rows, 16 * NQ));
+  hipLaunchKernelGGL((linear4_rows_kernel<E, NQ, NT, D>), grid, dim3(512), lds, s,
+                     (const typename E::type*)a.x, a.codes, a.scales, a.xs, (int)a.rows, (int)a.k,
+                     (int)a.n, (int)a.chunks, a);
+  return launch_check("linear4_rows_kernel");
+}
+
+template <typename E, int NQ, int U>
+static int launch_linear4_few_nt(const Lin4& a, hipStream_t s) {
+  // Columns a workgroup: so many that one round of workgroups, one to each of
+  // the 256 CUs, takes them, at most 64 (48 for two row tiles, whose registers
+  // end there).  8 rows of 4096 x 12288 (768 column tiles) by one, two, three
+  // and four tiles: 11.2, 11.4, 9.2 and 11.0 us; 16 of 4096 x 4096 (256): 5.9,
+  // 7.5, 8.9 and 10.6.
+  const int64_t tiles = (a.n + 15) / 16 * ((a.rows + 16 * NQ - 1) / (16 * NQ));
+  if (tiles <= 256) return launch_linear4_few<E, NQ, 1, U>(a, s);
+  if (tiles <= 512) return launch_linear4_few<E, NQ, 2, U>(a, s);
+  if constexpr (NQ == 1) {
+    if (tiles > 768) return launch_linear4_few<E, NQ, 4, U>(a, s);
+  }
+  return launch_linear4_few<E, NQ, 3, U>(a, s);
 }
 
 template <typename E>
 static int launch_linear4(const Lin4& a, hipStream_t s) {
-  if (a.rows <= 16) return launch_linear4_tile<E, 1, 1>(a, s);
-  if (a.rows <= 32) return launch_linear4_tile<E, 2, 2>(a, s);
-  return launch_linear4_tile<E, 4, 2>(a, s);
+  if (a.rows <= 16) return launch_linear4_few_nt<E, 1, 2>(a, s);
+  // float32 rows cost their split into terms, which the kernel for many rows
+  // shares between its waves: 40 x 256 x 18709 takes 8.6 us there, 12.4 here;
+  // 32 x 4096 x 12288 25 here, 34 there.
+  if (a.rows <= 32) return launch_linear4_few_nt<E, 2, E::terms == 3 ? 1 : 2>(a, s);
+  if constexpr (E::terms == 3) {
+    // (48 rows x 128 columns where that makes a round of workgroups, 40 x 256 x
+    // 18709: 8.6 us, 11.9 with 64 columns; otherwise 32 x 64, 128 x 4096 x 4096:
+    // 33 us, 45)
+    if (a.rows <= 48 && a.n > 64 * 256) return launch_linear4_rows<E, 3, 2, 2>(a, s);
+    return launch_linear4_rows<E, 2, 1, 4>(a, s);
+  } else {
+    // up to 64 rows as two blocks of 32: 64 x 2048 x 2048 6.6 us, 9.1 there
+    if (a.rows <= 64) return launch_linear4_few_nt<E, 2, 2>(a, s);
+    // 32 rows x 64 columns (128 x 4096 x 4096: 16 us, 22 with 64 rows), 64 rows
+    // where there is more than a round of them (64 x 4096 x 12288: 23 us, 26)
+    if ((a.n + 63) / 64 * ((a.rows + 63) / 64) >= 256) return launch_linear4_rows<E, 4, 1, 4>(a, s);
+    return launch_linear4_rows<E, 2, 1, 4>(a, s);
+  }
 }
 
 // -------------------------------------------------------------- host checks
@@ -326,7 +674,7 @@ QPH_API int qph_quantize4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t ro
                           int64_t row_stride, int64_t col_stride, void* codes, void* scales) {
   if (!dtype_valid(dtype)) return fail(QPH_EINVAL, "quantize4: unknown element type");
   if (rows < 0 || k <= 0) return fail(QPH_EINVAL, "quantize4: bad shape");
-  if (k > ((int64_t)1 << 31)) return fail(QPH_EUNSUPPORTED, "quantize4: more than 2^31 columns");
+  if (k > (1 << 30)) return fail(QPH_EUNSUPPORTED, "quantize4: more than 2^30 columns");
   if (rows && (!x || !codes || !scales)) return fail(QPH_EINVAL, "quantize4: NULL argument");
   if ((uintptr_t)codes % 16) return fail(QPH_EINVAL, "quantize4: codes are not 16-byte aligned");
   if (rows > ((int64_t)INT32_MAX * 256) / ((k + 127) / 128 * 4))
@@ -355,9 +703,9 @@ QPH_API int qph_linear4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t x_st
   if (rows && (!x || !codes || !scales || !y)) return fail(QPH_EINVAL, "linear4: NULL argument");
   if ((uintptr_t)codes % 16 || (uintptr_t)scales % 4)
     return fail(QPH_EINVAL, "linear4: codes are not 16-byte or scales not 4-byte aligned");
-  // grid limits, and addresses that 63 bits hold
-  if (n > ((int64_t)1 << 31) || k > ((int64_t)1 << 31) || rows > 65535 * (int64_t)16)
-    return fail(QPH_EUNSUPPORTED, "linear4: shape past 2^31 columns or 1048560 rows");
+  // columns, rows and k are counted in 32 bits, row tiles by the grid's second axis
+  if (n > (1 << 30) || k > (1 << 30) || rows > 65535 * 16)
+    return fail(QPH_EUNSUPPORTED, "linear4: more than 2^30 columns or inputs, or 1048560 rows");
   if (!ctx) return fail(QPH_EINVAL, "null context");
   if (rows == 0) return QPH_OK;
   Lin4 a{};

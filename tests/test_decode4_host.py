@@ -111,7 +111,7 @@ def test_bad_attention(lib, kw, code, text):
     (dict(page_table=None), "NULL argument"), (dict(lens=None), "NULL argument"),
     (dict(max_len=100000, max_pages=7000, workspace=None), "workspace"),
     (dict(max_len=100000, max_pages=7000, workspace_bytes=100), "workspace of 100 bytes"),
-    (dict(workspace=A + 2), "4-byte aligned"), (dict(), "null context"),
+    (dict(workspace=A + 8), "16-byte aligned"), (dict(), "null context"),
     (dict(tokens=0, q=None, out=None), "null context")])
 def test_bad_attention_call(lib, kw, text):
     refused(lib, lib.qph_attention_cache4(None, ctypes.byref(cache()), ctypes.byref(attn(**kw))),
@@ -163,8 +163,8 @@ def test_bad_linears(lib):
         refused(lib, call(**kw), EINVAL, "NULL argument")
     refused(lib, call(codes=A + 4), EINVAL, "aligned")
     refused(lib, call(scales=A + 2), EINVAL, "aligned")
-    refused(lib, call(n=1 << 40), EUNSUPPORTED, "2^31")
-    refused(lib, call(k=1 << 40), EUNSUPPORTED, "2^31")
+    refused(lib, call(n=1 << 40), EUNSUPPORTED, "2^30")
+    refused(lib, call(k=1 << 40), EUNSUPPORTED, "2^30")
     refused(lib, call(rows=1 << 30), EUNSUPPORTED, "rows")
     refused(lib, call(), EINVAL, "null context")
     refused(lib, call(rows=0, x=None, y=None), EINVAL, "null context")
@@ -176,7 +176,7 @@ def test_bad_quantize(lib):
     refused(lib, call(dtype=3), EINVAL, "element type")
     refused(lib, call(rows=-1), EINVAL, "bad shape")
     refused(lib, call(k=0), EINVAL, "bad shape")
-    refused(lib, call(k=1 << 40), EUNSUPPORTED, "2^31")
+    refused(lib, call(k=1 << 40), EUNSUPPORTED, "2^30")
     refused(lib, call(rows=1 << 50), EUNSUPPORTED, "blocks")
     refused(lib, call(x=None), EINVAL, "NULL argument")
     refused(lib, call(codes=A + 1), EINVAL, "aligned")

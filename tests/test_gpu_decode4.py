@@ -326,6 +326,51 @@ def test_linear_whole_numbers(gpu, dtype, rows, k, n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", [
+    (1, 96, 4100), (16, 130, 8200), (3, 40, 12300), (30, 257, 4112), (25, 384, 12290), (60, 300, 2500),
+    (48, 520, 16400), (47, 260, 16385), (66, 768, 8260), (129, 1100, 500), (70, 2600, 64)])
+def test_linear_wide(gpu, dtype, rows, k, n):
+    """Shapes that take more columns a workgroup, more rows, and more parts of
+    k than are in flight at once."""
+    from qppocr_amd import ops
+    print("linear4 wide", dtype, rows, k, n, flush=True)
+    t = getattr(gpu, dtype)
+    rng = np.random.default_rng(n + k)
+    def r(*s):
+        return gpu.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda().to(t)
+    w, x, b, e = ops.quantize4(r(k, n) / math.sqrt(k)), r(rows, k), r(n), r(rows, n)
+    want, tol = linear_reference(gpu, x, w, b, 0, e)
+    close(host(ops.linear4(x, w, b, 0, e)), want, tol + half_step(gpu, t, want) * 1.001, "linear4")
+
+
+@pytest.mark.parametrize("rows", [1, 20, 70])
+@pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** -22, 2.0 ** -12, 2.0 ** 12, 2.0 ** 20, 0.0])
+def test_linear_weights_of_any_size(gpu, rows, size):
+    """float16 x against weights inside and outside of float16's range, mixed
+    with ordinary ones and with blocks of zeros."""
+    from qppocr_amd import ops
+    print("linear4 sizes", rows, size, flush=True)
+    rng = np.random.default_rng(rows)
+    k, n = 700, 90
+    x = gpu.from_numpy((rng.standard_normal((rows, k)) * np.exp(rng.uniform(-9, 3, (rows, k))))
+                       .astype(np.float32)).cuda().half()
+    x[0, 5] = 2.0 ** -24                 # the smallest of all
+    for mixed in (False, True):
+        w = rng.standard_normal((k, n)) * size
+        if mixed:
+            w[64:96, ::3] = rng.standard_normal((32, 30)) * 0.1
+            w[300:400] = 0.0
+        w4 = ops.quantize4(gpu.from_numpy(w.astype(np.float32)).cuda())
+        want, tol = linear_reference(gpu, x, w4, None, 0, None)
+        got = ops.linear4(x, w4)
+        big = gpu.from_numpy(want).half()           # (past 65504: an infinity, as rounding gives)
+        assert (gpu.isinf(got).cpu() == gpu.isinf(big)).all() or size >= 2.0 ** 12
+        fine = np.abs(want) < 6.0e4
+        close(np.where(fine, host(got), 0), np.where(fine, want, 0),
+              tol + half_step(gpu, gpu.float16, want) * 1.001, f"size {size} {mixed}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_keeps_every_bit(gpu, dtype):
     """A weight that picks one input times 1: the input itself, all its bits,
     the largest and infinities among them."""
