@@ -88,7 +88,8 @@ class Cache4(ctypes.Structure):
 
 class Attn4(ctypes.Structure):
     """qph_attn4: the arguments of the attention over a 4-bit cache."""
-    _fields_ = [("q", P), ("out", P), ("lse", P), ("q_strides", I64 * 2), ("out_strides", I64 * 2),
+    _fields_ = [("q", P), ("out", P), ("lse", P), ("q_token", I64), ("q_head", I64),   # q_strides
+                ("out_token", I64), ("out_head", I64),                                 # out_strides
                 ("tokens", I64), ("batch", I64), ("page_table", P), ("table_stride", I64),
                 ("max_pages", I64), ("lens", P), ("starts", P), ("dtype", I32), ("heads", I32),
                 ("max_new", I32), ("max_len", I32), ("scale", F32), ("causal", I32),

@@ -465,36 +465,29 @@ _DTYPES = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat1
 _HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 _queued = {}
 _queue_lock = threading.Lock()
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(
+    torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-class _Queue:
-    """A library call on torch's current stream of a device, which does not wait.
+def _enqueue(device, fn, *args):
+    """fn(context, *args) on torch's current stream of a device, without waiting.
     The device's context for such calls takes the stream of each call under a
-    lock, since calls of several threads share it."""
-
-    __slots__ = ("device",)
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        stream = torch.cuda.current_stream(self.device).cuda_stream or _lib.STREAM_DEFAULT
-        _queue_lock.acquire()
-        try:
-            entry = _queued.get(self.device)
-            if entry is None:
-                entry = _queued[self.device] = [new_context(self.device), None]
-            if entry[1] != stream:
-                check(_lib.load().qph_ctx_set_stream(entry[0], stream))
-                entry[1] = stream
-            return entry[0]
-        except BaseException:
-            _queue_lock.release()
-            raise
-
-    def __exit__(self, kind, value, trace):
-        _queue_lock.release()
-        return False
+    lock, since calls of several threads share it.  (A decoder's step is some
+    hundred of these calls, whose host side decides where kernels are short:
+    with the stream's handle taken as it is and no objects made that a call can
+    do without, linear4 takes 7 us of it instead of 10.)"""
+    stream = _raw_stream(device) or _lib.STREAM_DEFAULT
+    with _queue_lock:
+        entry = _queued.get(device)
+        if entry is None:
+            entry = _queued[device] = [new_context(device), None]
+        if entry[1] != stream:
+            check(_lib.load().qph_ctx_set_stream(entry[0], stream))
+            entry[1] = stream
+        rc = fn(entry[0], *args)
+    if rc:
+        check(rc)
 
 
 def _dtype4(t, what):
@@ -504,18 +497,20 @@ def _dtype4(t, what):
     return d
 
 
-def _on(what, device, **tensors):
-    """Refuses tensors (None: absent) that do not lie on the device."""
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device != device):
-            raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
+def _on(what, device, name, t):
+    """Refuses a tensor that does not lie on the GPU `device`."""
+    if t.device != device or not t.is_cuda:
+        raise ValueError(f"{what}: {name} is on {t.device}, not on "
+                         f"{device if device.type == 'cuda' else 'a GPU'}")
 
 
-def _plain(what, name, t, dtype, shape):
-    """Refuses a tensor that is not contiguous, of the dtype and of the shape."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+def _plain(what, name, t, dtype, shape, device):
+    """Refuses a tensor that is not contiguous, of the dtype, of the shape and
+    on the device."""
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of shape "
                          f"{tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    _on(what, device, name, t)
 
 
 class Weight4:
@@ -528,12 +523,13 @@ class Weight4:
         if codes.dim() != 2 or k <= 0:
             raise ValueError("Weight4: codes [n, kp / 2] of k > 0 columns")
         n, kp = codes.shape[0], (k + 127) // 128 * 128
-        _on("Weight4", codes.device, codes=codes, scales=scales)
-        _plain("Weight4", "codes", codes, torch.uint8, (n, kp // 2))
-        _plain("Weight4", "scales", scales, torch.uint8, (n, kp // 32))
+        _plain("Weight4", "codes", codes, torch.uint8, (n, kp // 2), codes.device)
+        _plain("Weight4", "scales", scales, torch.uint8, (n, kp // 32), codes.device)
         if codes.data_ptr() % 16 or scales.data_ptr() % 4:
             raise ValueError("Weight4: codes are not 16-byte or scales not 4-byte aligned")
         self.codes, self.scales, self.n, self.k = codes, scales, n, int(k)
+        self.device, self._index = codes.device, codes.device.index
+        self._ptrs = codes.data_ptr(), scales.data_ptr()
 
 
 def quantize4(w):
@@ -545,13 +541,12 @@ def quantize4(w):
     if not k or not n:
         raise ValueError("quantize4: empty weight")
     d = _dtype4(w, "quantize4")
-    _on("quantize4", w.device, w=w)
+    _on("quantize4", w.device, "w", w)
     kp = (k + 127) // 128 * 128
     codes = torch.empty((n, kp // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((n, kp // 32), dtype=torch.uint8, device=w.device)
-    with _Queue(_dev(w)) as ctx:
-        check(_lib.load().qph_quantize4(ctx, w.data_ptr(), d, n, k, w.stride(1), w.stride(0),
-                                        codes.data_ptr(), scales.data_ptr()))
+    _enqueue(w.device.index, _lib.load().qph_quantize4, w.data_ptr(), d, n, k, w.stride(1),
+             w.stride(0), codes.data_ptr(), scales.data_ptr())
     return Weight4(codes, scales, k)
 
 
@@ -560,24 +555,29 @@ def linear4(x, w, bias=None, act_kind=ACT_NONE, residual=None):
     (float32, float16, bfloat16).  x's rows may lie apart (a slice of a packed
     projection); bias and residual are contiguous and of x's type."""
     d = _dtype4(x, "linear4")
-    if x.dim() < 1 or x.shape[-1] != w.k:
-        raise ValueError(f"linear4: x {tuple(x.shape)} against a weight of {w.k} inputs")
-    _on("linear4", w.codes.device, x=x, bias=bias, residual=residual)
-    shape = tuple(x.shape[:-1]) + (w.n,)
-    rows = x.numel() // w.k
-    x2 = x if x.dim() == 2 else x.reshape(rows, w.k)
-    if x2.stride(1) != 1 and w.k > 1:
+    k, n = w.k, w.n
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"linear4: x {tuple(x.shape)} against a weight of {k} inputs")
+    _on("linear4", w.device, "x", x)
+    if x.dim() == 2:
+        rows, x2 = x.shape[0], x
+        y = x.new_empty((rows, n))
+    else:
+        rows = x.numel() // k
+        x2 = x.reshape(rows, k)
+        y = x.new_empty(tuple(x.shape[:-1]) + (n,))
+    if x2.stride(1) != 1 and k > 1:
         x2 = x2.contiguous()
+    b = r = None
     if bias is not None:
-        _plain("linear4", "bias", bias, x.dtype, (w.n,))
+        _plain("linear4", "bias", bias, x.dtype, (n,), w.device)
+        b = bias.data_ptr()
     if residual is not None:
-        _plain("linear4", "residual", residual, x.dtype, shape)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    with _Queue(_dev(x)) as ctx:
-        check(_lib.load().qph_linear4(
-            ctx, x2.data_ptr(), d, x2.stride(0), w.codes.data_ptr(), w.scales.data_ptr(),
-            None if bias is None else bias.data_ptr(), rows, w.k, w.n, _act_ref(act_kind),
-            None if residual is None else residual.data_ptr(), y.data_ptr()))
+        _plain("linear4", "residual", residual, x.dtype, y.shape, w.device)
+        r = residual.data_ptr()
+    codes, scales = w._ptrs
+    _enqueue(w._index, _lib.load().qph_linear4, x2.data_ptr(), d, x2.stride(0), codes, scales, b,
+             rows, k, n, _act_ref(act_kind), r, y.data_ptr())
     return y
 
 
@@ -591,8 +591,6 @@ class Cache4:
         if k_codes.dim() != 4:
             raise ValueError("Cache4: codes [pages, heads, page size, dh / 2]")
         pages, heads, page, half = k_codes.shape
-        _on("Cache4", k_codes.device, k_codes=k_codes, k_scales=k_scales, v_codes=v_codes,
-            v_scales=v_scales)
         if 2 * half not in _HEAD_DIMS:
             raise ValueError(f"Cache4: head dimension {2 * half} is not one of {_HEAD_DIMS}")
         if page < 16 or page > 32768 or page & (page - 1):
@@ -602,11 +600,11 @@ class Cache4:
         for name, t, last in (("k_codes", k_codes, half), ("v_codes", v_codes, half),
                               ("k_scales", k_scales, half // 16),
                               ("v_scales", v_scales, half // 16)):
-            _plain("Cache4", name, t, torch.uint8, (pages, heads, page, last))
+            _plain("Cache4", name, t, torch.uint8, (pages, heads, page, last), k_codes.device)
         self.k_codes, self.k_scales = k_codes, k_scales
         self.v_codes, self.v_scales = v_codes, v_scales
         self.pages, self.heads, self.page_size, self.dh = pages, heads, page, 2 * half
-        self.device = k_codes.device
+        self.device, self._index = k_codes.device, k_codes.device.index
         self._c = _lib.Cache4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                               v_scales.data_ptr(), pages, page, heads, 2 * half)
         self._ref = ctypes.byref(self._c)
@@ -622,10 +620,14 @@ def cache4(pages, page_size, heads, dh, device="cuda"):
 
 
 def _rows4(what, name, t, cache, tokens, heads):
-    if tuple(t.shape) != (tokens, heads, cache.dh) or (t.stride(2) != 1 and t.numel()):
+    """Refuses a tensor that is not [tokens, heads, dh] with neighbouring elements
+    of a head, on the cache's device; its strides of a token and a head."""
+    strides = t.stride()
+    if t.shape != (tokens, heads, cache.dh) or (strides[2] != 1 and t.numel()):
         raise ValueError(f"{what}: {name} must be [{tokens}, {heads}, {cache.dh}] with neighbouring "
-                         f"elements of a head, not {tuple(t.shape)} of strides {t.stride()}")
-    return (_lib.I64 * 2)(t.stride(0), t.stride(1))
+                         f"elements of a head, not {tuple(t.shape)} of strides {strides}")
+    _on(what, cache.device, name, t)
+    return strides[:2]
 
 
 def cache4_write(cache, k, v, slots):
@@ -637,13 +639,11 @@ def cache4_write(cache, k, v, slots):
     if k.dim() != 3 or v.dtype != k.dtype:
         raise ValueError("cache4_write: k and v [tokens, heads, dh] of one type")
     n = k.shape[0]
-    _on("cache4_write", cache.device, k=k, v=v, slots=slots)
     ks = _rows4("cache4_write", "k", k, cache, n, cache.heads)
     vs = _rows4("cache4_write", "v", v, cache, n, cache.heads)
-    _plain("cache4_write", "slots", slots, torch.int64, (n,))
-    with _Queue(_dev(k)) as ctx:
-        check(_lib.load().qph_cache4_write(ctx, cache._ref, k.data_ptr(), v.data_ptr(), d, n, ks,
-                                           vs, slots.data_ptr()))
+    _plain("cache4_write", "slots", slots, torch.int64, (n,), cache.device)
+    _enqueue(cache._index, _lib.load().qph_cache4_write, cache._ref, k.data_ptr(), v.data_ptr(), d,
+             n, _dims(ks), _dims(vs), slots.data_ptr())
 
 
 def cache4_read(cache, slots, dtype=torch.float32, out=None):
@@ -655,20 +655,33 @@ def cache4_read(cache, slots, dtype=torch.float32, out=None):
     n = slots.shape[0]
     if out is None:
         shape = (n, cache.heads, cache.dh)
-        out = (torch.empty(shape, dtype=dtype, device=cache.device),
-               torch.empty(shape, dtype=dtype, device=cache.device))
-    k, v = out
+        k = torch.empty(shape, dtype=dtype, device=cache.device)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
     d = _dtype4(k, "cache4_read")
     if v.dtype != k.dtype:
         raise ValueError("cache4_read: k and v of one type")
-    _on("cache4_read", cache.device, k=k, v=v, slots=slots)
     ks = _rows4("cache4_read", "k", k, cache, n, cache.heads)
     vs = _rows4("cache4_read", "v", v, cache, n, cache.heads)
-    _plain("cache4_read", "slots", slots, torch.int64, (n,))
-    with _Queue(_dev(slots)) as ctx:
-        check(_lib.load().qph_cache4_read(ctx, cache._ref, k.data_ptr(), v.data_ptr(), d, n, ks,
-                                          vs, slots.data_ptr()))
+    _plain("cache4_read", "slots", slots, torch.int64, (n,), cache.device)
+    _enqueue(cache._index, _lib.load().qph_cache4_read, cache._ref, k.data_ptr(), v.data_ptr(), d, n,
+             _dims(ks), _dims(vs), slots.data_ptr())
     return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace4(pages, page, heads, dh, *sizes):
+    """qph_attention_cache4_workspace, which sees the sizes alone."""
+    c = _lib.Cache4(256, 256, 256, 256, pages, page, heads, dh)
+    a = _lib.Attn4()
+    (a.dtype, a.heads, a.tokens, a.batch, a.max_pages, a.max_new, a.max_len, a.causal, a.window,
+     a.starts) = sizes
+    a.scale = 1.0
+    size = ctypes.c_size_t()
+    check(_lib.load().qph_attention_cache4_workspace(ctypes.byref(c), ctypes.byref(a),
+                                                     ctypes.byref(size)))
+    return size.value
 
 
 def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=None, max_len=None,
@@ -690,45 +703,44 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
     d = _dtype4(q, what)
     if q.dim() != 3:
         raise ValueError(f"{what}: q [tokens, heads, dh]")
-    tokens, heads = q.shape[0], q.shape[1]
-    _on(what, cache.device, q=q, page_table=page_table, lens=lens, starts=starts, out=out)
+    tokens, heads, dh = q.shape
+    dev = cache.device
     qs = _rows4(what, "q", q, cache, tokens, heads)
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (
             page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError(f"{what}: page_table int32 [batch, pages], rows contiguous")
+    _on(what, dev, "page_table", page_table)
     batch, pages = page_table.shape
-    _plain(what, "lens", lens, torch.int32, (batch,))
+    _plain(what, "lens", lens, torch.int32, (batch,), dev)
+    at = None
     if starts is not None:
-        _plain(what, "starts", starts, torch.int32, (batch + 1,))
+        _plain(what, "starts", starts, torch.int32, (batch + 1,), dev)
         if max_new is None:
             raise ValueError(f"{what}: starts need max_new")
+        at = starts.data_ptr()
     elif batch and tokens % batch:
         raise ValueError(f"{what}: {tokens} tokens for {batch} sequences need starts")
-    elif batch:
-        if max_new is not None and max_new != tokens // batch:
-            raise ValueError(f"{what}: max_new {max_new} without starts, where every sequence "
-                             f"has {tokens // batch}")
-        max_new = tokens // batch
     else:
-        max_new = 0
+        each = tokens // batch if batch else 0
+        if max_new is not None and max_new != each and batch:
+            raise ValueError(f"{what}: max_new {max_new} without starts, where every sequence "
+                             f"has {each}")
+        max_new = each
     if max_len is None:
         max_len = min(pages * cache.page_size, 0x7fffff00)
     if out is None:
-        out = torch.empty((tokens, heads, cache.dh), dtype=q.dtype, device=q.device)
+        out = q.new_empty((tokens, heads, dh))
     elif out.dtype != q.dtype:
         raise ValueError(f"{what}: out is {out.dtype}, q {q.dtype}")
     os = _rows4(what, "out", out, cache, tokens, heads)
-    sums = torch.empty((tokens, heads), device=q.device) if lse else None
-    a = _lib.Attn4(q.data_ptr(), out.data_ptr(), None if sums is None else sums.data_ptr(), qs, os,
+    sums = torch.empty((tokens, heads), device=dev) if lse else None
+    max_new, max_len, window, causal = int(max_new), int(max_len), int(window), int(bool(causal))
+    size = _workspace4(cache.pages, cache.page_size, cache.heads, dh, d, heads, tokens, batch, pages,
+                       max_new, max_len, causal, window, None if at is None else 256)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    a = _lib.Attn4(q.data_ptr(), out.data_ptr(), None if sums is None else sums.data_ptr(), *qs, *os,
                    tokens, batch, page_table.data_ptr(), page_table.stride(0), pages,
-                   lens.data_ptr(), None if starts is None else starts.data_ptr(), d, heads,
-                   int(max_new), int(max_len), float(scale), int(bool(causal)), int(window), None,
-                   0)
-    lib, ref, size = _lib.load(), ctypes.byref(a), ctypes.c_size_t()
-    check(lib.qph_attention_cache4_workspace(cache._ref, ref, ctypes.byref(size)))
-    if size.value:
-        work = torch.empty(size.value, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), size.value
-    with _Queue(_dev(q)) as ctx:
-        check(lib.qph_attention_cache4(ctx, cache._ref, ref))
+                   lens.data_ptr(), at, d, heads, max_new, max_len, scale, causal, window,
+                   None if work is None else work.data_ptr(), size)
+    _enqueue(cache._index, _lib.load().qph_attention_cache4, cache._ref, ctypes.byref(a))
     return (out, sums) if lse else out

@@ -38,7 +38,7 @@ def attn(**kw):
              window=0, workspace=A, workspace_bytes=1 << 40)
     d.update(kw)
     a = _lib.Attn4(**d)
-    a.q_strides = a.out_strides = (ctypes.c_int64 * 2)(4 * 64, 64)
+    a.q_token, a.q_head, a.out_token, a.out_head = 4 * 64, 64, 4 * 64, 64
     return a
 
 
