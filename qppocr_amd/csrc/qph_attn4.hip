@@ -53,6 +53,11 @@ struct Attn4 {
 
 constexpr int64_t kMaxKeys = 0x7fffff00;     // of one sequence: positions stay in 31 bits
 
+// The running maximum of a wave with more rows moves only where a score passes
+// it by 2^8 (the terms are until then that much larger), so that the sums are
+// seldom scaled and the lanes of a column seldom compared.
+constexpr float kLazy = 8.0f;
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -123,9 +128,13 @@ __device__ __forceinline__ Pages find_pages(const Attn4& a, const PageIds& ids, 
 // A lane's part of 32 keys and values: W words of two keys, W bytes of eight
 // values, and their scales.
 template <int W>
-struct Tile {
-  unsigned kw[2][W], ks[2][Lane<W>::kblocks];
-  unsigned vw[8][Lane<W>::vwords], vs[8][Lane<W>::vblocks];
+struct KeyTile {
+  unsigned w[2][W], s[2][Lane<W>::kblocks];
+};
+
+template <int W>
+struct ValueTile {
+  unsigned w[8][Lane<W>::vwords], s[8][Lane<W>::vblocks];
 };
 
 // A lane's place in a tile's half, in bytes: the loads take a uniform base and
@@ -148,40 +157,38 @@ struct Place {
 };
 
 template <int W>
-__device__ __forceinline__ void load_tile(const Attn4& a, const Pages& pg, const Place<W>& at,
-                                          Tile<W>& t) {
+__device__ __forceinline__ void load_keys(const Attn4& a, const Pages& pg, const Place<W>& at,
+                                          KeyTile<W>& t) {
 #pragma unroll
   for (int u = 0; u < 2; u++) {
-    __builtin_memcpy(t.kw[u], a.kc + pg.row[u] * (16 * W) + at.k, 4 * W);
+    __builtin_memcpy(t.w[u], a.kc + pg.row[u] * (16 * W) + at.k, 4 * W);
     const unsigned char* s = a.ks + pg.row[u] * W;
-    t.ks[u][0] = s[at.ks];
-    if constexpr (Lane<W>::kblocks > 1) t.ks[u][1] = s[at.ks1];
+    t.s[u][0] = s[at.ks];
+    if constexpr (Lane<W>::kblocks > 1) t.s[u][1] = s[at.ks1];
   }
+}
+
+template <int W>
+__device__ __forceinline__ void load_values(const Attn4& a, const Pages& pg, const Place<W>& at,
+                                            ValueTile<W>& t) {
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     const unsigned char* p = a.vc + pg.row[e / 4] * (16 * W) + at.v;
     const unsigned char* s = a.vs + pg.row[e / 4] * W;
     constexpr unsigned row = 16 * W;
     const unsigned r = e % 4;
-    if constexpr (W == 1) {
-      t.vw[e][0] = p[r * row];
-    } else if constexpr (W == 2) {
-      t.vw[e][0] = *(const unsigned short*)(p + r * row);
-    } else if constexpr (W == 6) {
-      unsigned long long v;
-      __builtin_memcpy(&v, p + r * row, 8);
-      t.vw[e][0] = (unsigned)v;
-      t.vw[e][1] = (unsigned)(v >> 32);
-    } else {
-      __builtin_memcpy(t.vw[e], p + r * row, sizeof t.vw[e]);
-    }
-    t.vs[e][0] = s[at.vs + r * W];
-    if constexpr (Lane<W>::vblocks > 1) t.vs[e][1] = s[at.vs1 + r * W];
+    if constexpr (W == 1) t.w[e][0] = p[r * row];
+    else if constexpr (W == 2) t.w[e][0] = *(const unsigned short*)(p + r * row);
+    else __builtin_memcpy(t.w[e], p + r * row, sizeof t.w[e]);
+    t.s[e][0] = s[at.vs + r * W];
+    if constexpr (Lane<W>::vblocks > 1) t.s[e][1] = s[at.vs1 + r * W];
   }
 }
 
+// (Registers: three waves a SIMD hide more of the loads than the last of them
+// are worth; 32 sequences of 4096 keys, float16: 43 us so, 48 with two.)
 template <typename E, int W, int NQ, int WS>
-__global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
+__global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) void attn4_kernel(Attn4 a) {
   constexpr int T = E::terms, PT = T < 2 ? 2 : T;
   constexpr int DH = 32 * W;
   extern __shared__ float lds[];
@@ -277,18 +284,18 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
 
     bool careful = false;      // second run: value blocks of NaN are kept from the rows that do not see them
-    auto compute = [&](Tile<W>& tl, const Pages& pg, int j0) __attribute__((always_inline)) {
+    auto compute = [&](const KeyTile<W>& kt, ValueTile<W>& vt, const Pages& pg, int j0) __attribute__((always_inline)) {
       f32x4 s[2][NQ];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const int g0 = W * kg / 4;
-        const float s0 = scale_of_byte(tl.ks[u][0]);
-        const float s1 = Lane<W>::kblocks > 1 ? scale_of_byte(tl.ks[u][Lane<W>::kblocks - 1]) : s0;
+        const float s0 = scale_of_byte(kt.s[u][0]);
+        const float s1 = Lane<W>::kblocks > 1 ? scale_of_byte(kt.s[u][Lane<W>::kblocks - 1]) : s0;
 #pragma unroll
         for (int q = 0; q < NQ; q++) s[u][q] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int n = 0; n < W; n++) {
-          const bf16x8 kf = fp4_word(tl.kw[u][n], (W * kg + n) / 4 == g0 ? s0 : s1);
+          const bf16x8 kf = fp4_word(kt.w[u][n], (W * kg + n) / 4 == g0 ? s0 : s1);
 #pragma unroll
           for (int q = 0; q < NQ; q++)
 #pragma unroll
@@ -315,10 +322,11 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
         float mx = s[0][q][0];
 #pragma unroll
         for (int e = 1; e < 8; e++) mx = fmaxf(mx, s[e / 4][q][e % 4]);
-        const float top = fmaxf(m[q], column_max(mx) * c);
-        const float sub = top == -INFINITY ? 0.0f : top;
-        if (__any(top > m[q])) {
-          const float keep = exp2_(m[q] - sub);
+        float top = m[q];
+        if constexpr (NQ == 1) top = fmaxf(top, column_max(mx) * c);
+        if (__any(NQ == 1 ? top > m[q] : mx * c > m[q] + kLazy)) {
+          if constexpr (NQ > 1) top = fmaxf(top, column_max(mx) * c);
+          const float keep = exp2_(m[q] - (top == -INFINITY ? 0.0f : top));
           m[q] = top;
           l[q] *= keep;
 #pragma unroll
@@ -326,6 +334,7 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
 #pragma unroll
             for (int r = 0; r < 4; r++) o[q][x][r] *= keep;
         }
+        const float sub = m[q] == -INFINITY ? 0.0f : m[q];
         float p[8], sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -347,7 +356,7 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
           bf16x8 nan;
 #pragma unroll
           for (int e = 0; e < 8; e++)
-            nan[e] = (half ? tl.vs[e][Lane<W>::vblocks - 1] : tl.vs[e][0]) == 255 ? (__bf16)1.0f : (__bf16)0.0f;
+            nan[e] = (half ? vt.s[e][Lane<W>::vblocks - 1] : vt.s[e][0]) == 255 ? (__bf16)1.0f : (__bf16)0.0f;
 #pragma unroll
           for (int q = 0; q < NQ; q++) {
             const f32x4 hit = mfma16(nan, ones[q], f32x4{0, 0, 0, 0});
@@ -360,7 +369,7 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
         for (int e = 0; e < 8; e++)
 #pragma unroll
           for (int i = 0; i < Lane<W>::vblocks; i++)
-            if (tl.vs[e][i] == 255) tl.vs[e][i] = 0;
+            if (vt.s[e][i] == 255) vt.s[e][i] = 0;
       }
       // values
       float vsc[8][Lane<W>::vblocks];
@@ -368,16 +377,16 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
       for (int e = 0; e < 8; e++)
 #pragma unroll
         for (int i = 0; i < Lane<W>::vblocks; i++)
-          vsc[e][i] = scale_of_byte(tl.vs[e][i]);
+          vsc[e][i] = scale_of_byte(vt.s[e][i]);
       if constexpr (Lane<W>::odd) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           if constexpr (W == 3) {
-            tl.vw[e][0] >>= place.shift;
+            vt.w[e][0] >>= place.shift;
           } else {
-            const unsigned long long v = ((unsigned long long)tl.vw[e][1] << 32 | tl.vw[e][0]) >> place.shift;
-            tl.vw[e][0] = (unsigned)v;
-            tl.vw[e][1] = (unsigned)(v >> 32);
+            const unsigned long long v = ((unsigned long long)vt.w[e][1] << 32 | vt.w[e][0]) >> place.shift;
+            vt.w[e][0] = (unsigned)v;
+            vt.w[e][1] = (unsigned)(v >> 32);
           }
         }
       }
@@ -388,7 +397,7 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
         for (int e = 0; e < 8; e++) {
           const bool half = Lane<W>::vblocks > 1 && (W * li + y) / 16 != W * li / 16;
           const float sc = half ? vsc[e][Lane<W>::vblocks - 1] : vsc[e][0];
-          const unsigned w = tl.vw[e][y / 4];
+          const unsigned w = vt.w[e][y / 4];
           pr[e] = y % 4 == 0 ? fp4_pair<0>(w, sc) : y % 4 == 1 ? fp4_pair<1>(w, sc)
                 : y % 4 == 2 ? fp4_pair<2>(w, sc) : fp4_pair<3>(w, sc);
         }
@@ -408,7 +417,9 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
       }
     };
 
-    // Tiles of 32 keys, the next one's loads in flight while one is computed.
+    // Tiles of 32 keys, the next one's loads in flight while one is computed (with
+    // more rows a wave the values' come late, behind the keys' products: their
+    // registers are needed, and there is enough to compute until then).
     // A value block of NaN must not reach the rows that do not see its key, but
     // 0 * NaN does: where the result holds a NaN, the keys are walked again
     // with such blocks as zeros, and the rows that see them get their NaN from
@@ -424,23 +435,30 @@ __global__ __launch_bounds__(256) void attn4_kernel(Attn4 a) {
       }
       int j0 = klo + (WS == 4 ? 32 * wave : 0);
       if (j0 < khi) {
-        Tile<W> ta, tb;
+        constexpr bool late = NQ > 1;
+        KeyTile<W> ka, kb;
+        ValueTile<W> va, vb;
         Pages pa = find_pages(a, page_ids(a, table, j0, khi), j0, h), pb;
-        load_tile<W>(a, pa, place, ta);
+        load_keys<W>(a, pa, place, ka);
+        if (!late) load_values<W>(a, pa, place, va);
         PageIds ids = page_ids(a, table, j0 + step, khi);
         while (true) {
+          if (late) load_values<W>(a, pa, place, va);
           pb = find_pages(a, ids, j0 + step, h);
-          load_tile<W>(a, pb, place, tb);
+          load_keys<W>(a, pb, place, kb);
+          if (!late) load_values<W>(a, pb, place, vb);
           ids = page_ids(a, table, j0 + 2 * step, khi);
           __builtin_amdgcn_sched_barrier(0);
-          compute(ta, pa, j0);
+          compute(ka, va, pa, j0);
           j0 += step;
           if (j0 >= khi) break;
+          if (late) load_values<W>(a, pb, place, va);
           pa = find_pages(a, ids, j0 + step, h);
-          load_tile<W>(a, pa, place, ta);
+          load_keys<W>(a, pa, place, ka);
+          if (!late) load_values<W>(a, pa, place, va);
           ids = page_ids(a, table, j0 + 2 * step, khi);
           __builtin_amdgcn_sched_barrier(0);
-          compute(tb, pb, j0);
+          compute(kb, late ? va : vb, pb, j0);
           j0 += step;
           if (j0 >= khi) break;
         }

@@ -56,7 +56,7 @@ struct Cache4Io {
   int64_t tokens;
   void *k, *v;
   int64_t kt, kh, vt, vh;     // strides of a token and a head, in elements
-  int per;                    // tokens a workgroup
+  int per;                    // tokens a workgroup takes at once
 };
 
 // Where head h of a cached token starts, in heads' rows.
@@ -64,9 +64,10 @@ __device__ __forceinline__ int64_t cache4_row(int64_t slot, int shift, unsigned 
   return ((((slot >> shift) * heads + h) << shift) + (slot & (((int64_t)1 << shift) - 1)));
 }
 
-// A word of codes (eight elements) per thread; the four threads of a block of
-// 32 share its largest magnitude by two swaps inside a quad.
-template <typename E>
+// A word of codes (eight elements) per thread and token, U tokens (per * U a
+// workgroup) in flight; the four threads of a block of 32 share its largest
+// magnitude by two swaps inside a quad (a quad is of one token).
+template <typename E, int U>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Io a) {
   const unsigned units = a.heads * a.words, total = units * (unsigned)a.per;
   const bool second = blockIdx.y != 0;
@@ -76,27 +77,38 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Io a) {
   unsigned char* scales = second ? a.vs : a.ks;
   for (unsigned u = threadIdx.x; u < total; u += blockDim.x) {
     const unsigned lt = u / units, w = u % units, h = w / a.words, c = w % a.words;
-    const int64_t t = (int64_t)blockIdx.x * a.per + lt;
-    if (t >= a.tokens) break;                 // (a quad is of one token)
-    const int64_t slot = a.slots[t];
-    if (slot < 0 || slot >= a.slots_n) continue;
-    float v[8];
-    load8<E>(x + t * xt + h * xh + c * 8, v);
-    unsigned top = 0;
+    const int64_t t0 = (int64_t)blockIdx.x * (a.per * U) + lt;
+    int64_t slot[U];
+    float v[U][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    top = max(top, (unsigned)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xf, 0xf, true));  // lane ^ 1
-    top = max(top, (unsigned)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xf, 0xf, true));  // lane ^ 2
-    const int e = fp4_exponent(top);
-    const bool bad = e == -1000;
-    const int64_t row = cache4_row(slot, a.shift, a.heads, h);
-    ((unsigned*)codes)[row * a.words + c] =
-        bad ? 0u : fp4_encode8(v, scale_of_byte((unsigned)(e + 127)));
-    if (c % 4 == 0) scales[row * (a.words / 4) + c / 4] = (unsigned char)(bad ? 255 : e + 127);
+    for (int i = 0; i < U; i++) {
+      const int64_t t = t0 + i * a.per;
+      slot[i] = -1;
+      if (t >= a.tokens) continue;
+      slot[i] = a.slots[t];
+      load8<E>(x + t * xt + h * xh + c * 8, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      if (slot[i] < 0 || slot[i] >= a.slots_n) continue;
+      unsigned top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+      top = max(top, (unsigned)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xf, 0xf, true));  // lane ^ 1
+      top = max(top, (unsigned)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xf, 0xf, true));  // lane ^ 2
+      const int e = fp4_exponent(top);
+      const bool bad = e == -1000;
+      const int64_t row = cache4_row(slot[i], a.shift, a.heads, h);
+      ((unsigned*)codes)[row * a.words + c] =
+          bad ? 0u : fp4_encode8(v[i], scale_of_byte((unsigned)(e + 127)));
+      if (c % 4 == 0) scales[row * (a.words / 4) + c / 4] = (unsigned char)(bad ? 255 : e + 127);
+    }
   }
 }
 
-template <typename E>
+// A word of codes per thread and token, U tokens (per * U a workgroup) in
+// flight: the slots, then the codes and scales, then the rows.
+template <typename E, int U>
 __global__ __launch_bounds__(256) void cache4_read_kernel(Cache4Io a) {
   const unsigned units = a.heads * a.words, total = units * (unsigned)a.per;
   const bool second = blockIdx.y != 0;
@@ -106,21 +118,30 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Cache4Io a) {
   const unsigned char* scales = second ? a.vs : a.ks;
   for (unsigned u = threadIdx.x; u < total; u += blockDim.x) {
     const unsigned lt = u / units, w = u % units, h = w / a.words, c = w % a.words;
-    const int64_t t = (int64_t)blockIdx.x * a.per + lt;
-    if (t >= a.tokens) break;
-    const int64_t slot = a.slots[t];
-    float v[8];
-    if (slot < 0 || slot >= a.slots_n) {
+    const int64_t t0 = (int64_t)blockIdx.x * (a.per * U) + lt;
+    int64_t row[U];
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = 0.0f;
-    } else {
-      const int64_t row = cache4_row(slot, a.shift, a.heads, h);
-      const bf16x8 b = fp4_word(((const unsigned*)codes)[row * a.words + c],
-                                scale_of_byte(scales[row * (a.words / 4) + c / 4]));
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = (float)b[i];
+    for (int i = 0; i < U; i++) {
+      const int64_t slot = a.slots[min(t0 + i * a.per, a.tokens - 1)];
+      row[i] = slot < 0 || slot >= a.slots_n ? -1 : cache4_row(slot, a.shift, a.heads, h);
     }
-    store8<E>(y + t * yt + h * yh + c * 8, v);
+    unsigned code[U], scale[U];
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      const int64_t r = max(row[i], (int64_t)0);
+      code[i] = ((const unsigned*)codes)[r * a.words + c];
+      scale[i] = scales[r * (a.words / 4) + c / 4];
+    }
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      const int64_t t = t0 + i * a.per;
+      if (t >= a.tokens) break;
+      const bf16x8 b = fp4_word(row[i] < 0 ? 0u : code[i], scale_of_byte(row[i] < 0 ? 127u : scale[i]));
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = (float)b[e];
+      store8<E>(y + t * yt + h * yh + c * 8, v);
+    }
   }
 }
 
@@ -143,19 +164,6 @@ struct Lin4 {
 __device__ __forceinline__ float act4_apply(float v, const Act& a) {
   if (a.kind == 1) return a.c3 * v * ((a.c2 - 1.0f) + erfcf(-v * a.inv_c1));
   return act_apply(v, a);
-}
-
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-template <int B>
-__device__ __forceinline__ unsigned fp4_pair_f16(unsigned w, float scale) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, B));
-}
-
-__device__ __forceinline__ f16x8 fp4_word_f16(unsigned w, float scale) {
-  const u32x4 v = {fp4_pair_f16<0>(w, scale), fp4_pair_f16<1>(w, scale), fp4_pair_f16<2>(w, scale),
-                   fp4_pair_f16<3>(w, scale)};
-  return __builtin_bit_cast(f16x8, v);
 }
 
 // A block whose numbers are exact in float16: scale bytes 104 to 140 (6 2^13
@@ -640,15 +648,20 @@ static int cache4_io(qph_ctx* ctx, const qph_cache4* c, void* k, void* v, int32_
   a.kt = ks[0]; a.kh = ks[1]; a.vt = vs[0]; a.vh = vs[1];
   const unsigned units = a.heads * a.words;
   a.per = (int)std::max(1u, 256u / units);
-  const int64_t groups = (tokens + a.per - 1) / a.per;
+  // Tokens in flight a thread: four where workgroups are many (reading 65521
+  // tokens of 8 x 128: 69 us, 94 with one and 67 with eight; 300000 of 1 x 64:
+  // 18, 20 and 21), one where they are few.
+  const int flight = tokens / a.per >= 8192 ? 4 : 1;
+  const int64_t groups = (tokens + a.per * flight - 1) / (a.per * flight);
   if (groups > INT32_MAX) return fail(QPH_EUNSUPPORTED, w + ": too many tokens for one call");
   OnDevice dev(ctx);
   QPH_TRY(dev.rc());
   const dim3 grid((unsigned)groups, 2);
-#define QPH_LAUNCH(E)                                                                     \
-  do {                                                                                    \
-    if (write) hipLaunchKernelGGL(cache4_write_kernel<E>, grid, dim3(256), 0, ctx->stream, a); \
-    else hipLaunchKernelGGL(cache4_read_kernel<E>, grid, dim3(256), 0, ctx->stream, a);   \
+#define QPH_LAUNCH(E)                                                                              \
+  do {                                                                                             \
+    auto fn = write ? (flight == 4 ? cache4_write_kernel<E, 4> : cache4_write_kernel<E, 1>)        \
+                    : (flight == 4 ? cache4_read_kernel<E, 4> : cache4_read_kernel<E, 1>);         \
+    hipLaunchKernelGGL(fn, grid, dim3(256), 0, ctx->stream, a);                                    \
   } while (0)
   if (dtype == QPH_F32) QPH_LAUNCH(F32);
   else if (dtype == QPH_F16) QPH_LAUNCH(F16);
