@@ -644,17 +644,29 @@ static Attn4Plan attn4_plan(const qph_cache4* c, const qph_attn4* p) {
                            ? std::min<int64_t>(p->max_len, (int64_t)p->window + p->max_new + 31)
                            : p->max_len;
   const int64_t seqs = (int64_t)p->batch * c->heads;
-  const bool many = p->dtype != QPH_F32 ? c->dh <= 128 : c->dh <= 64;
-  if (rows <= 16) { r.nq = 1; r.ws = 4; }
-  else if (many && (rows + 63) / 64 * seqs >= 512) { r.nq = 2; r.ws = 1; }
-  else { r.nq = 1; r.ws = rows * seqs >= 64 * 512 ? 1 : 4; }
+  // Waves with 32 rows of their own where they fill the card and their registers
+  // do (up to 128 elements a head, 64 in float32), waves of a workgroup that
+  // share 16 rows and split the keys otherwise.  us with 32 rows and with 16,
+  // bfloat16: a chunk of 1024 tokens, 32 / 8 heads of 128 over 4000 keys (512
+  // waves) 138 and 147, of 512 tokens over 2000 (256 waves) 72 and 48, 16 of 64
+  // tokens, 16 / 4 heads of 64 (512 waves of little work) 56 and 32.
+  const bool many = (p->dtype != QPH_F32 ? c->dh <= 128 : c->dh <= 64) && rows >= 1024 &&
+                    (rows + 63) / 64 * seqs >= 512;
+  r.nq = many ? 2 : 1;
+  r.ws = many ? 1 : 4;
   const int64_t tiles = (rows + 16 * r.nq - 1) / (16 * r.nq);
   r.row_tiles = (int)std::min<int64_t>(std::max<int64_t>(1, r.ws == 4 ? tiles : (tiles + 3) / 4), 1 << 20);
   r.splits = 1;
   r.chunk = (int64_t)1 << 40;
   const int64_t blocks = r.row_tiles * seqs;
-  if (r.ws == 4 && blocks < 2048 && keys > 512) {
-    int64_t n = std::min<int64_t>({(2048 + blocks - 1) / blocks, (keys + 255) / 256, 64});
+  // Splits along the keys: up to six workgroups a CU, of 512 keys or more (of
+  // 256 where that leaves CUs without one).  us with a bound of 1024, this one
+  // and 2048 workgroups: 64 sequences of 0 to 16384 keys, 8 heads, 160, 138 and
+  // 155; 128 of 1000 to 2000 keys 55, 57 and 65.  512 keys against 256: 64
+  // sequences of 512 to 1024 keys 18 and 25 to 30; one of 2000 keys 12 and 11.
+  const int64_t least = keys / 512 >= (255 + blocks) / blocks ? 512 : 256;
+  if (r.ws == 4 && 2 * blocks <= 1536 && keys > 2 * least) {
+    int64_t n = std::min<int64_t>({1536 / blocks, (keys + least - 1) / least, 64});
     r.chunk = ((keys + n - 1) / n + 127) / 128 * 128;
     n = (keys + r.chunk - 1) / r.chunk;
     if (n > 1) r.splits = (int)n;
@@ -678,7 +690,6 @@ static int launch_attn4_w(const Attn4& a, const Attn4Plan& p, hipStream_t s) {
   if constexpr (W <= (E::terms == 3 ? 2 : 4)) {
     if (p.nq == 2) return launch_attn4_one<E, W, 2, 1>(a, s);
   }
-  if (p.ws == 1) return launch_attn4_one<E, W, 1, 1>(a, s);
   return launch_attn4_one<E, W, 1, 4>(a, s);
 }
 

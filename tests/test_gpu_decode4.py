@@ -586,6 +586,52 @@ def test_attention_many_rows(gpu, dtype, dh):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dh", [32, 64, 96, 128])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 40), (False, 0)])
+def test_attention_rows_of_their_own(gpu, dtype, dh, causal, window):
+    """Chunks long enough that a wave takes 32 rows alone (float32: up to 64
+    elements): odd lengths, a hole in the pages, a key's and a value's block of
+    NaN, garbage behind the last token, rows before the first key."""
+    from qppocr_amd import ops
+    rng = np.random.default_rng(dh + window)
+    heads, group, page = 8, 16, 32
+    news, lens = [70, 64, 0, 66, 69], [71, 200, 40, 64, 150]
+    pages = sum((n + page - 1) // page for n in lens) + 1
+    c = make_cache(gpu, rng, pages, page, heads, dh)
+    table = tables(rng, pages, page, lens)
+    table[4][1] = -1                                   # keys 32 to 63 of the last sequence
+    for p, n in ((table[0][2], 71 % page), (table[1][6], 200 % page)):
+        c.k_scales[p, :, n:], c.v_scales[p, :, n:] = 255, 255
+    c.v_scales[table[1][4], 3, 20, 0] = 255            # value 148 of head 3, sequence 1
+    c.k_scales[table[4][3], 5, 10, 0] = 255            # key 106 of head 5, sequence 4
+    print("attention rows of their own", dtype, dh, causal, window, flush=True)
+    q = gpu.from_numpy(rng.standard_normal((sum(news), heads * group, dh)).astype(np.float32))
+    q = q.cuda().to(getattr(gpu, dtype))
+    st = [0] + list(np.cumsum(news))
+    y, sums = ops.attention_cache4(q, c, gpu.tensor(table, dtype=gpu.int32, device="cuda"),
+                                   gpu.tensor(lens, dtype=gpu.int32, device="cuda"), dh ** -0.5,
+                                   starts=gpu.tensor(st, dtype=gpu.int32, device="cuda"), max_new=70,
+                                   causal=causal, window=window, lse=True)
+    y, sums, qd = host(y), host(sums), host(q)
+    k, v = numbers(c)
+    terms = {"float32": 3, "float16": 2, "bfloat16": 1}[dtype]
+    for b, i in ((0, 0), (0, 35), (0, 69), (1, 0), (1, 11), (1, 12), (1, 13), (1, 63), (3, 0), (3, 1),
+                 (3, 2), (3, 40), (3, 65), (4, 0), (4, 24), (4, 25), (4, 26), (4, 68)):
+        p = lens[b] - news[b] + i
+        pos = np.arange(lens[b])
+        pg = np.array(table[b])[pos // page]
+        see = pg >= 0
+        if causal:
+            see &= pos <= p
+        if window:
+            see &= pos > p - window
+        want, tol, (lse, ltol) = attend_row(qd[st[b] + i], k[pg[see], pos[see] % page],
+                                            v[pg[see], pos[see] % page], dh ** -0.5, terms, group)
+        close(y[st[b] + i], want, tol + half_step(gpu, q.dtype, want) * 1.001, f"token {b} {i}")
+        close(sums[st[b] + i], lse, ltol, f"lse of token {b} {i}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_long(gpu, dtype):
     """Contexts that many workgroups share, and bounds that are too small or
     too large for them."""
