@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
   const int64_t rows = (int64_t)news * a.group;
   const ScalarI32 table = (ScalarI32)(a.table + b * a.table_stride);
   const int first = len - news;          // position of the first new token
-  const int base = a.window > 0 ? max(0, first - a.window + 1) & ~31 : 0;
+  const int base = a.window > 0 ? (int)max((int64_t)0, (int64_t)first - a.window + 1) & ~31 : 0;
   const int from = (int)min(base + split * a.chunk, (int64_t)room);
   const int to = split == a.splits - 1 ? room : (int)min(from + a.chunk, (int64_t)room);
 
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
       tok[q] = t0 + i;
       const int pos = first + i;
       hi[q] = a.causal ? min(len, max(pos + 1, 0)) : len;
-      lo[q] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      lo[q] = a.window > 0 ? (int)max((int64_t)0, (int64_t)pos - a.window + 1) : 0;
       if (!live[q]) lo[q] = hi[q] = 0;
       if (lo[q] < hi[q]) { wlo = min(wlo, lo[q]); whi = max(whi, hi[q]); }
       const typename E::type* p = (const typename E::type*)a.q + tok[q] * a.qt + head[q] * a.qh;
@@ -314,6 +314,17 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
               const bool see = pg.there[u] && j >= max(lo[q], from) && j < min(hi[q], to);
               if (!see) s[u][q][r] = -INFINITY;
             }
+        // the values of keys that no row sees, whatever stands there, are zeros
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int j = j0 + 16 * (e / 4) + 4 * kg + e % 4;
+          if (!pg.there[e / 4] || j < wlo || j >= khi) {
+#pragma unroll
+            for (int i = 0; i < Lane<W>::vblocks; i++) vt.s[e][i] = 127;
+#pragma unroll
+            for (int i = 0; i < Lane<W>::vwords; i++) vt.w[e][i] = 0;
+          }
+        }
       }
       // running maximum, exponentials
       bf16x8 pf[NQ][PT];
@@ -356,7 +367,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
           bf16x8 nan;
 #pragma unroll
           for (int e = 0; e < 8; e++)
-            nan[e] = (half ? vt.s[e][Lane<W>::vblocks - 1] : vt.s[e][0]) == 255 ? (__bf16)1.0f : (__bf16)0.0f;
+            nan[e] = (half ? vt.s[e][Lane<W>::vblocks - 1] : vt.s[e][0]) > 252 ? (__bf16)1.0f : (__bf16)0.0f;
 #pragma unroll
           for (int q = 0; q < NQ; q++) {
             const f32x4 hit = mfma16(nan, ones[q], f32x4{0, 0, 0, 0});
@@ -369,7 +380,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
         for (int e = 0; e < 8; e++)
 #pragma unroll
           for (int i = 0; i < Lane<W>::vblocks; i++)
-            if (vt.s[e][i] == 255) vt.s[e][i] = 0;
+            if (vt.s[e][i] > 252) vt.s[e][i] = 0;
       }
       // values
       float vsc[8][Lane<W>::vblocks];
@@ -423,7 +434,8 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
     // A value block of NaN must not reach the rows that do not see its key, but
     // 0 * NaN does: where the result holds a NaN, the keys are walked again
     // with such blocks as zeros, and the rows that see them get their NaN from
-    // a product of ones.
+    // a product of ones.  (So do scale bytes 253 and 254, whose numbers overflow;
+    // the format has none.)
     const int step = WS == 4 ? 128 : 32;
     while (true) {
 #pragma unroll

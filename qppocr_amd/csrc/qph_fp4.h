@@ -134,6 +134,13 @@ __device__ __forceinline__ void split8(const float v[8], bf16x8 out[T]) {
   }
 }
 
+// Between the stores and loads of a wave's own part of LDS that pass data between
+// its lanes: they are carried out in order, and must stay in order.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // The scale exponent of a block whose largest magnitude has these bits: the
 // smallest power of two that puts it at 6 or below.  -1000 for a block with
 // an infinity or a NaN.

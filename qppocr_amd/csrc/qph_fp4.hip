@@ -370,6 +370,7 @@ __global__ __launch_bounds__(512) void linear4_few_kernel(const typename E::type
     // the columns' loads meet in a bank
 #pragma unroll
     for (int u = 0; u < U; u++) {
+      wave_order();
 #pragma unroll
       for (int q = 0; q < NQ; q++)
 #pragma unroll
@@ -378,6 +379,7 @@ __global__ __launch_bounds__(512) void linear4_few_kernel(const typename E::type
           const int r = step * i + lane / pieces;
           *(u32x4*)(part + ((q * 16 + r) * pieces + ((lane % pieces) ^ r)) * 16) = xv[u][q][i];
         }
+      wave_order();
       u32x4 wu[NT];
       unsigned fu[NT];
 #pragma unroll

@@ -702,6 +702,74 @@ def test_attention_nan_stays_with_its_rows(gpu, dtype, dh):
     assert np.isnan(y).all() and np.isnan(s).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_over_memory_never_written(gpu, dtype):
+    """A pool whose unwritten tokens hold any bytes at all (scales that overflow
+    among them): only the written ones count, in short and in split walks."""
+    from qppocr_amd import ops
+    rng = np.random.default_rng(31)
+    t = getattr(gpu, dtype)
+    for dh, heads, group, news, lens, window in ((64, 2, 3, [1, 1, 1], [17, 64, 31], 0),
+                                                 (128, 1, 4, [5, 2], [1500, 1239], 0),
+                                                 (96, 1, 1, [3], [70], 40),
+                                                 (32, 8, 16, [66, 65, 64, 64], [66, 90, 70, 100], 0)):
+        print("attention never written", dtype, dh, lens, flush=True)
+        page = 64
+        pages = sum((n + page - 1) // page for n in lens) + 2
+        c = ops.cache4(pages, page, heads, dh)
+        for x in (c.k_codes, c.k_scales, c.v_codes, c.v_scales):
+            x.copy_(gpu.from_numpy(rng.integers(0, 256, x.shape, dtype=np.uint8)))
+        for x in (c.k_scales, c.v_scales):
+            x[:, :, 1::2] = gpu.from_numpy(rng.integers(250, 256, x[:, :, 1::2].shape, dtype=np.uint8)).cuda()
+        table = tables(rng, pages, page, lens)
+        for b, n in enumerate(lens):
+            pos = np.arange(n)
+            slots = np.array(table[b])[pos // page] * page + pos % page
+            kv = gpu.from_numpy(rng.standard_normal((2, n, heads, dh)).astype(np.float32)).cuda().to(t)
+            ops.cache4_write(c, kv[0], kv[1], gpu.from_numpy(slots.astype(np.int64)).cuda())
+        q = gpu.from_numpy(rng.standard_normal((sum(news), heads * group, dh)).astype(np.float32)).cuda().to(t)
+        y, s = check_attention(gpu, c, q, table, lens, dh ** -0.5, news, window=window)
+        assert np.isfinite(y).all() and np.isfinite(s).all()
+
+
+def test_attention_widest_window(gpu):
+    """The largest window hides nothing, rows before the first key included."""
+    rng = np.random.default_rng(33)
+    c = make_cache(gpu, rng, 3, 32, 1, 64)
+    q = gpu.from_numpy(rng.standard_normal((9, 2, 64)).astype(np.float32)).cuda()
+    for causal in (False, True):
+        check_attention(gpu, c, q, [[2, 0]], [4], 0.2, [9], causal, (1 << 31) - 1)
+
+
+def test_first_call_inside_a_capture(gpu):
+    """Nothing is set up by a first call that a capture would not allow: a new
+    process captures its first call of either kind (after torch's own start)."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from qppocr_amd import ops
+x = torch.randn(2, 64, device="cuda")
+w = ops.Weight4(torch.zeros((8, 64), dtype=torch.uint8, device="cuda") + 0x22,
+                torch.zeros((8, 4), dtype=torch.uint8, device="cuda") + 127, 64)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = ops.linear4(x, w)
+for _ in range(3):
+    x.normal_()
+    g.replay()
+    torch.cuda.synchronize()
+    want = x.double().sum(1, keepdim=True).expand(2, 8)
+    assert (y.double() - want).abs().max() < 1e-4, (y, want)
+print("captured")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout[-500:] + r.stderr[-1500:]
+
+
 def test_attention_strides_and_rows_left_alone(gpu):
     """q out of a packed projection, out with a stride of its own; rows before
     the first and behind the last sequence keep what they hold."""
