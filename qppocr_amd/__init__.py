@@ -2,7 +2,8 @@
 
 Modules:
   _lib   ctypes binding of libqppocr_hip.so (include/qppocr_hip.h)
-  ops    operator API mirroring qppocr-kernels (conv2d, sgemm, softmax_last_dim, ...)
+  ops    operator API mirroring qppocr-kernels (conv2d, sgemm, softmax_last_dim, ...);
+         4-bit linears, key / value cache and attention over it for decoders
   nets   det / rec graphs of the synthetic workloads and HipSession (DeviceSession)
   build  compiles csrc/*.hip for gfx950
 """

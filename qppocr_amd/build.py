@@ -36,7 +36,9 @@ CFLAGS = [
 
 # The accumulators of the 4-bit kernels are also read and scaled by VALU
 # instructions, which cannot reach the accumulation registers: without this the
-# compiler copies them there and back in every step.
+# compiler copies them there and back in every step.  Their smallest calls are
+# latency from end to end, so the first arguments come in registers with the
+# wave rather than by a load it has to wait for.
 EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm",
              "-amdgpu-kernarg-preload-count=16"] for f in ("qph_fp4.hip", "qph_attn4.hip")}
 

@@ -17,7 +17,6 @@
 
 namespace qph {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -31,7 +30,6 @@ struct F32 { typedef float type; static constexpr int terms = 3; };
 struct F16 { typedef _Float16 type; static constexpr int terms = 2; };
 struct BF16 { typedef __bf16 type; static constexpr int terms = 1; };
 
-inline size_t dtype_size(int32_t d) { return d == QPH_F32 ? 4 : 2; }
 inline bool dtype_valid(int32_t d) { return d == QPH_F32 || d == QPH_F16 || d == QPH_BF16; }
 
 // Makes the context's device current for one call and puts the caller's back.
@@ -88,12 +86,6 @@ __device__ __forceinline__ void load8(const typename E::type* p, float v[8]) {
   __builtin_memcpy(t, p, sizeof t);
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = (float)t[i];
-}
-
-template <typename E>
-__device__ __forceinline__ void load8_upto(const typename E::type* p, int n, float v[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = i < n ? (float)p[i] : 0.0f;
 }
 
 template <typename E>

@@ -584,8 +584,8 @@ static int launch_linear4(const Lin4& a, hipStream_t s) {
   // 32 x 4096 x 12288 25 here, 34 there.
   if (a.rows <= 32) return launch_linear4_few_nt<E, 2, E::terms == 3 ? 1 : 2>(a, s);
   if constexpr (E::terms == 3) {
-    // (48 rows x 128 columns where that makes a round of workgroups, 40 x 256 x
-    // 18709: 8.6 us, 11.9 with 64 columns; otherwise 32 x 64, 128 x 4096 x 4096:
+    // (48 rows x 128 columns where 64 columns are more than a round of workgroups,
+    // 40 x 256 x 18709: 8.6 us, 11.9 with 64 columns; otherwise 32 x 64, 128 x 4096 x 4096:
     // 33 us, 45)
     if (a.rows <= 48 && a.n > 64 * 256) return launch_linear4_rows<E, 3, 2, 2>(a, s);
     return launch_linear4_rows<E, 2, 1, 4>(a, s);
