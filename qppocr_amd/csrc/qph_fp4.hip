@@ -406,18 +406,22 @@ __global__ __launch_bounds__(512) void linear4_few_kernel(const typename E::type
       }, acc);
     }
   }
+  // (four columns' place in a row turns with the row where the rows would
+  // otherwise start in a part of the banks only)
+  constexpr int turn = NT % 2 ? 0 : 16 * NT - 4;
   float* red = (float*)lds4;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NT; i++)
 #pragma unroll
     for (int q = 0; q < NQ; q++)
-      *(f32x4*)&red[(((wave * NQ + q) * 16 + li) * NT + i) * 16 + 4 * kg] = acc[i][q];
+      *(f32x4*)&red[((wave * NQ + q) * 16 + li) * (16 * NT) + ((16 * i + 4 * kg) ^ (4 * li & turn))] = acc[i][q];
   __syncthreads();
   constexpr int tile = NQ * 16 * NT * 16;
   for (int i = 4 * threadIdx.x; i < tile; i += 4 * blockDim.x) {
-    f32x4 v = *(const f32x4*)&red[i];
-    for (int w = 1; w < waves; w++) v += *(const f32x4*)&red[w * tile + i];
+    const int at = i ^ (4 * (i / (16 * NT)) & turn);
+    f32x4 v = *(const f32x4*)&red[at];
+    for (int w = 1; w < waves; w++) v += *(const f32x4*)&red[w * tile + at];
     linear4_store<E>(a, r0 + i / (16 * NT), j0 + i % (16 * NT), v);
   }
 }
@@ -520,7 +524,8 @@ __global__ __launch_bounds__(512) void linear4_rows_kernel(const typename E::typ
       load(it + d + D, s[d]);
     }
   }
-  // the two halves' sums
+  // the two halves' sums; four columns' place in a row turns with the row, or
+  // all rows of a tile would be in the same banks
   float* red = (float*)lds4;
   __syncthreads();
   constexpr int cols = 64 * NT, tile = 16 * NQ * cols;
@@ -528,10 +533,12 @@ __global__ __launch_bounds__(512) void linear4_rows_kernel(const typename E::typ
   for (int i = 0; i < NT; i++)
 #pragma unroll
     for (int q = 0; q < NQ; q++)
-      *(f32x4*)&red[wk * tile + (q * 16 + li) * cols + (wn * NT + i) * 16 + 4 * kg] = acc[i][q];
+      *(f32x4*)&red[wk * tile + (q * 16 + li) * cols + (((wn * NT + i) * 16 + 4 * kg) ^ (4 * li))] = acc[i][q];
   __syncthreads();
-  for (int i = 4 * tid; i < tile; i += 2048)
-    linear4_store<E>(a, r0 + i / cols, j0 + i % cols, *(f32x4*)&red[i] + *(f32x4*)&red[tile + i]);
+  for (int i = 4 * tid; i < tile; i += 2048) {
+    const int at = i ^ (4 * (i / cols & 15));
+    linear4_store<E>(a, r0 + i / cols, j0 + i % cols, *(f32x4*)&red[at] + *(f32x4*)&red[tile + at]);
+  }
 }
 
 template <typename E, int NQ, int NT, int U>
@@ -578,24 +585,34 @@ static int launch_linear4_few_nt(const Lin4& a, hipStream_t s) {
 
 template <typename E>
 static int launch_linear4(const Lin4& a, hipStream_t s) {
+  constexpr bool f32 = E::terms == 3;
+  // up to 16 rows: 16 x 4096 x 32768 22 us (float32 33), 33 (52) by more rows' kernel
   if (a.rows <= 16) return launch_linear4_few_nt<E, 1, 2>(a, s);
-  // float32 rows cost their split into terms, which the kernel for many rows
-  // shares between its waves: 40 x 256 x 18709 takes 8.6 us there, 12.4 here;
-  // 32 x 4096 x 12288 25 here, 34 there.
-  if (a.rows <= 32) return launch_linear4_few_nt<E, 2, E::terms == 3 ? 1 : 2>(a, s);
-  if constexpr (E::terms == 3) {
-    // (48 rows x 128 columns where 64 columns are more than a round of workgroups,
-    // 40 x 256 x 18709: 8.6 us, 11.9 with 64 columns; otherwise 32 x 64, 128 x 4096 x 4096:
-    // 33 us, 45)
-    if (a.rows <= 48 && a.n > 64 * 256) return launch_linear4_rows<E, 3, 2, 2>(a, s);
-    return launch_linear4_rows<E, 2, 1, 4>(a, s);
+  // More rows cost their turning and, in float32, their split into terms in
+  // every workgroup here; the other kernel shares them between more columns,
+  // with less of the weights in flight.  So here while one round of workgroups
+  // does: 64 x 4096 x 4096 10.7 us, 15.8 there, 32 x 4096 x 12288 in float32 25
+  // and 34; past it 64 x 4096 x 8192 is 22.1 and 16.8, 64 x 4096 x 32768 60 and
+  // 35, 32 x 4096 x 32768 in float32 67 and 53.
+  const bool round = (a.n + 47) / 48 * ((a.rows + 31) / 32) <= 256;
+  const bool round_32x64 = (a.n + 63) / 64 * ((a.rows + 31) / 32) <= 256;
+  // (two-byte rows that 32 hold also where that one needs more than a round of
+  // its smallest workgroups: 20 x 1024 x 18709 7.6 and 11.6 us, 32 x 4096 x 32768
+  // 32.0 and 33.9, but 32 x 4096 x 16384 21.9 and 17.0)
+  if (a.rows <= (f32 ? 32 : 64) && (round || (!f32 && a.rows <= 32 && !round_32x64)))
+    return launch_linear4_few_nt<E, 2, f32 ? 1 : 2>(a, s);
+  // Then the smallest workgroups that one round takes: 32 rows x 64 columns (128
+  // x 4096 x 4096 16 us, 22 with 64 rows; in float32 35, 48 with 48 rows x 128
+  // columns), 64 x 64 (256 x 4096 x 4096 23.4; 26.5 with 32 rows, 31.5 with 128
+  // columns).  Past that the ones that do most with what they load: 64 x 128
+  // (2048 x 4096 x 12288 343 us, 470 with 64 columns), in float32 48 x 128 (779
+  // us, 1425 with 32 x 64).
+  if (round_32x64) return launch_linear4_rows<E, 2, 1, 4>(a, s);
+  if constexpr (f32) {
+    return launch_linear4_rows<E, 3, 2, 2>(a, s);
   } else {
-    // up to 64 rows as two blocks of 32: 64 x 2048 x 2048 6.6 us, 9.1 there
-    if (a.rows <= 64) return launch_linear4_few_nt<E, 2, 2>(a, s);
-    // 32 rows x 64 columns (128 x 4096 x 4096: 16 us, 22 with 64 rows), 64 rows
-    // where there is more than a round of them (64 x 4096 x 12288: 23 us, 26)
-    if ((a.n + 63) / 64 * ((a.rows + 63) / 64) >= 256) return launch_linear4_rows<E, 4, 1, 4>(a, s);
-    return launch_linear4_rows<E, 2, 1, 4>(a, s);
+    if ((a.n + 63) / 64 * ((a.rows + 63) / 64) <= 256) return launch_linear4_rows<E, 4, 1, 4>(a, s);
+    return launch_linear4_rows<E, 4, 2, 2>(a, s);
   }
 }
 

@@ -327,6 +327,24 @@ def test_linear_whole_numbers(gpu, dtype, rows, k, n):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,k,n", [
+    (130, 300, 8330), (200, 70, 5500), (64, 200, 16500), (70, 520, 6100), (32, 260, 13000),
+    (20, 140, 17000), (321, 1100, 4227), (64, 1030, 6200), (49, 513, 16421), (9, 700, 16999)])
+def test_linear_more_than_a_round(gpu, dtype, rows, k, n):
+    """Rows and columns at both sides of where the workgroups of a form no
+    longer go into one round."""
+    from qppocr_amd import ops
+    print("linear4 rounds", dtype, rows, k, n, flush=True)
+    t = getattr(gpu, dtype)
+    rng = np.random.default_rng(n + k)
+    def r(*s):
+        return gpu.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda().to(t)
+    w, x, b, e = ops.quantize4(r(k, n) / math.sqrt(k)), r(rows, k + 1)[:, 1:], r(n), r(rows, n)
+    want, tol = linear_reference(gpu, x, w, b, 0, e)
+    close(host(ops.linear4(x, w, b, 0, e)), want, tol + half_step(gpu, t, want) * 1.001, "linear4")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", [
     (1, 96, 4100), (16, 130, 8200), (3, 40, 12300), (30, 257, 4112), (25, 384, 12290), (60, 300, 2500),
     (48, 520, 16400), (47, 260, 16385), (66, 768, 8260), (129, 1100, 500), (70, 2600, 64)])
 def test_linear_wide(gpu, dtype, rows, k, n):
