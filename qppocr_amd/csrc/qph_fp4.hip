@@ -177,7 +177,7 @@ __device__ __forceinline__ bool fits_f16(unsigned s, u32x4 w) {
 // neighbouring k of one column, one block: 16 bytes of codes and one scale, so
 // it needs the 32 neighbouring elements of a row of x beside them.  x comes in
 // whole lines and is turned in LDS; straight from memory each load would touch
-// 64 lines (32 rows of 4096 x 12288: 41 us so, 24 through LDS).  float16 x
+// 64 lines (an early form, 32 rows of 4096 x 12288: 41 us so, 24 through LDS).  float16 x
 // against weights that are exact in float16 (any of ordinary size) is one
 // float16 product of full precision, otherwise x is split into bfloat16 terms.
 
