@@ -578,7 +578,10 @@ static int launch_linear4_few_nt(const Lin4& a, hipStream_t s) {
   if (tiles <= 256) return launch_linear4_few<E, NQ, 1, U>(a, s);
   if (tiles <= 512) return launch_linear4_few<E, NQ, 2, U>(a, s);
   if constexpr (NQ == 1) {
-    if (tiles > 768) return launch_linear4_few<E, NQ, 4, U>(a, s);
+    // past 1024 tiles as many rounds as four tiles make, but even ones: 1 x 4096
+    // x 20000 by three 15.1 us, by four 17.5, 16 x 256 x 18709 5.1 and 5.8
+    const int64_t round = (tiles + 1023) / 1024 * 256;
+    if (tiles > 3 * round) return launch_linear4_few<E, NQ, 4, U>(a, s);
   }
   return launch_linear4_few<E, NQ, 3, U>(a, s);
 }
