@@ -733,7 +733,7 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
     elif out.dtype != q.dtype:
         raise ValueError(f"{what}: out is {out.dtype}, q {q.dtype}")
     os = _rows4(what, "out", out, cache, tokens, heads)
-    sums = torch.empty((tokens, heads), device=dev) if lse else None
+    sums = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if lse else None
     max_new, max_len, window, causal = int(max_new), int(max_len), int(window), int(bool(causal))
     size = _workspace4(cache.pages, cache.page_size, cache.heads, dh, d, heads, tokens, batch, pages,
                        max_new, max_len, causal, window, None if at is None else 256)

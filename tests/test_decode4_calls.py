@@ -1,0 +1,65 @@
+"""The Python calls of the 4-bit operators as the library gets them, on the host:
+the device's check and the library's call are replaced, the tensors are host
+tensors, and nothing is computed."""
+import os
+
+import pytest
+import torch
+
+from qppocr_amd import _lib, ops
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+class Lib:
+    """Every entry point's name in its place, but the plan's (it needs no GPU)."""
+
+    def __init__(self, real):
+        self.qph_attention_cache4_workspace = real.qph_attention_cache4_workspace
+
+    def __getattr__(self, name):
+        return name
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The library's calls as they come: (device, name, arguments)."""
+    if not os.path.exists(_lib.LIB_PATH):
+        from qppocr_amd import build
+        build.build()
+    lib, got = Lib(_lib.load()), []
+    monkeypatch.setattr(ops, "_on", lambda *a: None)
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(ops, "_enqueue", lambda device, fn, *a: got.append((device, fn, a)))
+    return got
+
+
+def cache(pages=4, page=16, heads=2, dh=64):
+    return ops.cache4(pages, page, heads, dh, device="cpu")
+
+
+def attend(c, tokens=3, heads=4, dtype=torch.float32, pages=4, **kw):
+    q = kw.pop("q", None)
+    q = torch.zeros((tokens, heads, c.dh), dtype=dtype) if q is None else q
+    return ops.attention_cache4(q, c, torch.zeros((tokens, pages), dtype=torch.int32),
+                                torch.ones(tokens, dtype=torch.int32), 0.125, **kw)
+
+
+@pytest.mark.parametrize("default", [torch.float32, torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_buffer_has_its_own_type(calls, default, dtype):
+    """What the calls allocate does not follow torch's default type: the sums of
+    the attention are float32 always."""
+    was = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        c = cache()
+        out, sums = attend(c, dtype=dtype, lse=True)
+        assert out.dtype == dtype and sums.dtype == torch.float32 and tuple(sums.shape) == (3, 4)
+        k, v = ops.cache4_read(c, torch.zeros(5, dtype=torch.int64), dtype)
+        assert k.dtype == v.dtype == dtype
+        w = ops.quantize4(torch.zeros((64, 8), dtype=dtype))
+        assert w.codes.dtype == w.scales.dtype == torch.uint8
+        assert ops.linear4(torch.zeros((2, 64), dtype=dtype), w).dtype == dtype
+    finally:
+        torch.set_default_dtype(was)
