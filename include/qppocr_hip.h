@@ -390,7 +390,8 @@ QPH_API int qph_cache4_read(qph_ctx* ctx, const qph_cache4* cache, void* k, void
  * are left as they were.  max_new and max_len (host) bound the sequences' new
  * and cached tokens; they choose the work's split, and longer ones only run
  * slower.  lens are cut at max_pages pages.  Scores, sums and the running
- * maximum are float32, keys and values exact, the probabilities kept to 16
+ * maximum are float32 (scores of any finite size; one past float32's range
+ * makes its row NaN), keys and values exact, the probabilities kept to 16
  * bits (24 for float32) in the second product.
  * page_table, lens and starts are device memory.  The workspace (device, of
  * qph_attention_cache4_workspace bytes for the same arguments, which depend on

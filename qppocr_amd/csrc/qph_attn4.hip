@@ -62,6 +62,31 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The maximum is kept as a score m; the terms are 2^(s c - m c), c = |scale|
+// log2 e.  With m c rounded, a term is one fused operation and all terms of the
+// row are off by the same factor 2^r, r up to half a unit of m c, which the
+// sums share.  Past this bound 2^r is more than 2^(1/32), later out of float32's
+// range, and the row's terms are 2^((s - m) c), whose largest is 1: such a row
+// is walked again with its m known.  (In every tile both cost more: 6 to 8 % of a
+// chunk's time as a branch or as a difference ahead of the product.)
+constexpr float kFar = 1048576.0f;
+
+__device__ __forceinline__ bool is_far(float mc) { return fabsf(mc) >= kFar; }
+
+// log2 of the factor from sums with the maximum `was` to sums with `top`; was <= top,
+// top not -infinity.
+__device__ __forceinline__ float rescale(float was, float top, float c) {
+  const float wc = was * c, tc = top * c;
+  if (is_far(wc)) return is_far(tc) ? (was - top) * c : __builtin_fmaf(was, c, -tc);
+  return is_far(tc) ? -__builtin_fmaf(top, c, -wc) : wc - tc;
+}
+
+// log of the sum of the row's exponentials; l the sum of its terms.
+__device__ __forceinline__ float log_sum(float m, float l, float scale) {
+  const float mc = m * (scale * kLog2e);
+  return (is_far(mc) ? m * scale : mc * kLn2) + logf(l);
+}
+
 // The larger over the four lanes of one column (lane ^ 16, lane ^ 32).
 __device__ __forceinline__ float column_max(float v) {
   u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -223,7 +248,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
   for (int64_t tile = WS == 4 ? rt0 : (int64_t)rt0 * 4 + wave; tile * 16 * NQ < rows;
        tile += (int64_t)a.row_tiles * (WS == 4 ? 1 : 4)) {
     // (a row has seen a key if and only if its sum is not 0: the largest score's
-    // term is 1, and NaN is not 0 either)
+    // term is 1 or near it, and NaN is not 0 either)
     // rows of this wave: query fragments, visible keys [lo, hi)
     bf16x8 qf[NQ][T][W];
     int64_t tok[NQ];
@@ -268,7 +293,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
 
     const Place<W> place(li, kg);
     f32x4 o[NQ][2 * W];
-    float m[NQ], l[NQ];
+    float m[NQ], l[NQ], shift[NQ];     // shift: what a second walk takes off the scores
 
     // minimum and maximum of the live rows' borders: between them a tile needs no masks
     int all_lo = 0, all_hi = khi;
@@ -283,7 +308,9 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
     all_lo = __builtin_amdgcn_readfirstlane(max(all_lo, from));
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
 
-    bool careful = false;      // second run: value blocks of NaN are kept from the rows that do not see them
+    // (the margin of the running maximum as a score; it vanishes beside a far one)
+    const float lazy = fminf(kLazy / c, 3.4e38f);
+    bool careful = false;      // second run
     auto compute = [&](const KeyTile<W>& kt, ValueTile<W>& vt, const Pages& pg, int j0) __attribute__((always_inline)) {
       f32x4 s[2][NQ];
 #pragma unroll
@@ -303,7 +330,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
         }
       }
       // masks, only where a border lies in the tile or a page is none
-      if (j0 < all_lo || j0 + 32 > all_hi || !(pg.there[0] && pg.there[1])) {
+      if (careful || j0 < all_lo || j0 + 32 > all_hi || !(pg.there[0] && pg.there[1])) {
 #pragma unroll
         for (int q = 0; q < NQ; q++)
 #pragma unroll
@@ -312,7 +339,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
             for (int r = 0; r < 4; r++) {
               const int j = j0 + 16 * u + 4 * kg + r;
               const bool see = pg.there[u] && j >= max(lo[q], from) && j < min(hi[q], to);
-              if (!see) s[u][q][r] = -INFINITY;
+              s[u][q][r] = see ? s[u][q][r] - shift[q] : -INFINITY;
             }
         // the values of keys that no row sees, whatever stands there, are zeros
 #pragma unroll
@@ -334,10 +361,16 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
 #pragma unroll
         for (int e = 1; e < 8; e++) mx = fmaxf(mx, s[e / 4][q][e % 4]);
         float top = m[q];
-        if constexpr (NQ == 1) top = fmaxf(top, column_max(mx) * c);
-        if (__any(NQ == 1 ? top > m[q] : mx * c > m[q] + kLazy)) {
-          if constexpr (NQ > 1) top = fmaxf(top, column_max(mx) * c);
-          const float keep = exp2_(m[q] - (top == -INFINITY ? 0.0f : top));
+        bool grows;
+        if constexpr (NQ == 1) {
+          top = fmaxf(top, column_max(mx));
+          grows = top > m[q];
+        } else {
+          grows = mx > m[q] + lazy;
+        }
+        if (__any(grows)) {
+          if constexpr (NQ > 1) top = fmaxf(top, column_max(mx));
+          const float keep = exp2_(m[q] * c - (top == -INFINITY ? 0.0f : top * c));
           m[q] = top;
           l[q] *= keep;
 #pragma unroll
@@ -345,11 +378,11 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
 #pragma unroll
             for (int r = 0; r < 4; r++) o[q][x][r] *= keep;
         }
-        const float sub = m[q] == -INFINITY ? 0.0f : m[q];
+        const float mc = m[q] == -INFINITY ? 0.0f : m[q] * c;
         float p[8], sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          p[e] = exp2_(__builtin_fmaf(s[e / 4][q][e % 4], c, -sub));
+          p[e] = exp2_(__builtin_fmaf(s[e / 4][q][e % 4], c, -mc));
           sum += p[e];
         }
         l[q] += sum;
@@ -431,16 +464,23 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
     // Tiles of 32 keys, the next one's loads in flight while one is computed (with
     // more rows a wave the values' come late, behind the keys' products: their
     // registers are needed, and there is enough to compute until then).
-    // A value block of NaN must not reach the rows that do not see its key, but
-    // 0 * NaN does: where the result holds a NaN, the keys are walked again
-    // with such blocks as zeros, and the rows that see them get their NaN from
-    // a product of ones.  (So do scale bytes 253 and 254, whose numbers overflow;
-    // the format has none.)
+    // Keys are walked a second time, for what would cost the first one more in
+    // every tile.  A value block of NaN must not reach the rows that do not see
+    // its key, but 0 * NaN does: where the result holds a NaN, such blocks are
+    // zeros the second time, and the rows that see them get their NaN from a
+    // product of ones.  (So do scale bytes 253 and 254, whose numbers overflow;
+    // the format has none.)  And a row whose maximum ends past kFar has it taken
+    // off its scores; one whose maximum was so far past it on the way that a sum
+    // overflowed (the rescaling has made that a NaN) starts with its last maximum.
     const int step = WS == 4 ? 128 : 32;
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+      m[q] = -INFINITY;
+      shift[q] = 0.0f;
+    }
     while (true) {
 #pragma unroll
       for (int q = 0; q < NQ; q++) {
-        m[q] = -INFINITY;
         l[q] = 0.0f;
 #pragma unroll
         for (int x = 0; x < 2 * W; x++) o[q][x] = f32x4{0, 0, 0, 0};
@@ -475,16 +515,27 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
           if (j0 >= khi) break;
         }
       }
-      bool nan = false;
+      if (careful) break;
 #pragma unroll
-      for (int q = 0; q < NQ; q++)
+      for (int q = 0; q < NQ; q++) {
+        careful |= m[q] != -INFINITY && is_far(m[q] * c);
 #pragma unroll
         for (int x = 0; x < 2 * W; x++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) nan |= o[q][x][r] != o[q][x][r];
-      if (careful || !__any(nan)) break;
-      careful = true;
+          for (int r = 0; r < 4; r++) careful |= o[q][x][r] != o[q][x][r];
+      }
+      careful = __any(careful);
+      if (!careful) break;
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        const float sum = column_sum(l[q]);
+        const bool far = m[q] != -INFINITY && is_far(m[q] * c);
+        shift[q] = far ? m[q] : 0.0f;
+        m[q] = far ? 0.0f : sum != sum ? m[q] : -INFINITY;
+      }
     }
+#pragma unroll
+    for (int q = 0; q < NQ; q++) m[q] += shift[q];
 
     // the sums of a row: over the lanes of its column, then (WS = 4) over the
     // workgroup's waves, in their order
@@ -517,10 +568,9 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
           wm[w] = ml[((w * NQ + q) * 16 + li) * 2];
           top = fmaxf(top, wm[w]);
         }
-        const float sub = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-          wm[w] = exp2_(wm[w] - sub);
+          wm[w] = top == -INFINITY ? 0.0f : exp2_(rescale(wm[w], top, c));
           sum += wm[w] * ml[((w * NQ + q) * 16 + li) * 2 + 1];
         }
         m[q] = top;
@@ -557,7 +607,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
       } else {
         const float inv = l[q] == 0.0f ? 0.0f : 1.0f / l[q];
         if (a.lse && kg == 0 && (WS == 1 || wave == 0))
-          a.lse[at] = l[q] == 0.0f ? -INFINITY : m[q] * kLn2 + logf(l[q]);
+          a.lse[at] = l[q] == 0.0f ? -INFINITY : log_sum(m[q], l[q], fabsf(a.scale));
 #pragma unroll
         for (int r = 0; r < NR; r++) {
           typename E::type* p = (typename E::type*)a.out + tok[q] * a.ot + head[q] * a.oh +
@@ -596,7 +646,7 @@ __global__ __launch_bounds__(256) void attn4_join_kernel(Attn4 a, int dh) {
     float top = m;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    const float w = exp2_(m - (top == -INFINITY ? 0.0f : top));
+    const float w = top == -INFINITY ? 0.0f : exp2_(rescale(m, top, fabsf(a.scale) * kLog2e));
     float sum = w * l;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
@@ -620,7 +670,7 @@ __global__ __launch_bounds__(256) void attn4_join_kernel(Attn4 a, int dh) {
       }
     }
     if (a.lse && lane == 0 && (JW == 1 || wave == 0))
-      a.lse[row] = some ? top * kLn2 + logf(sum) : -INFINITY;
+      a.lse[row] = some ? log_sum(top, sum, fabsf(a.scale)) : -INFINITY;
     const float inv = some ? 1.0f / sum : 0.0f;
     typename E::type* out = (typename E::type*)a.out + t * a.ot + (row % qheads) * a.oh;
     if constexpr (JW == 4) {
