@@ -20,6 +20,7 @@
 // that become row i of product m.  Codes turn into bfloat16 in registers, one
 // instruction for two.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "qph_fp4.h"
@@ -53,9 +54,10 @@ struct Attn4 {
 
 constexpr int64_t kMaxKeys = 0x7fffff00;     // of one sequence: positions stay in 31 bits
 
-// The running maximum of a wave with more rows moves only where a score passes
-// it by 2^8 (the terms are until then that much larger), so that the sums are
-// seldom scaled and the lanes of a column seldom compared.
+// The maximum of a wave with more rows is a bound, set 2^8 past the largest score
+// so far and moved where a score passes it, so that the sums are seldom scaled
+// and the lanes of a column seldom compared.  (Past it, not at it: no term is
+// above 1, and the sums overflow no sooner than they would with the maximum.)
 constexpr float kLazy = 8.0f;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -67,7 +69,7 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // row are off by the same factor 2^r, r up to half a unit of m c, which the
 // sums share.  Past this bound 2^r is more than 2^(1/32), later out of float32's
 // range, and the row's terms are 2^((s - m) c), whose largest is 1: such a row
-// is walked again with its m known.  (In every tile both cost more: 6 to 8 % of a
+// is walked again with its m known.  (In every tile both cost more: 5 to 7 % of a
 // chunk's time as a branch or as a difference ahead of the product.)
 constexpr float kFar = 1048576.0f;
 
@@ -308,8 +310,8 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
     all_lo = __builtin_amdgcn_readfirstlane(max(all_lo, from));
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
 
-    // (the margin of the running maximum as a score; it vanishes beside a far one)
-    const float lazy = fminf(kLazy / c, 3.4e38f);
+    // (the bound's distance as a score; it vanishes beside a far one)
+    const float lazy = fminf(kLazy / c, FLT_MAX);
     bool careful = false;      // second run
     auto compute = [&](const KeyTile<W>& kt, ValueTile<W>& vt, const Pages& pg, int j0) __attribute__((always_inline)) {
       f32x4 s[2][NQ];
@@ -366,10 +368,13 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
           top = fmaxf(top, column_max(mx));
           grows = top > m[q];
         } else {
-          grows = mx > m[q] + lazy;
+          grows = mx > m[q];
         }
         if (__any(grows)) {
-          if constexpr (NQ > 1) top = fmaxf(top, column_max(mx));
+          if constexpr (NQ > 1) {
+            const float most = column_max(mx);
+            if (most > top) top = fminf(most + lazy, fmaxf(most, FLT_MAX));
+          }
           const float keep = exp2_(m[q] * c - (top == -INFINITY ? 0.0f : top * c));
           m[q] = top;
           l[q] *= keep;

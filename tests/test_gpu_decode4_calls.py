@@ -210,3 +210,33 @@ def test_attention_far_scores_before_ordinary_ones(gpu, dtype, form, common):
         close(y, want, tol + half_step(gpu, t, want) * 1.001, name)
         ref = z.max() + np.log(p.sum())
         close(np.array(lse), np.array(ref), 2.0 ** -22 * abs(ref) + 2.0 ** -21 + d, name + " lse")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_attention_values_near_the_largest_number(gpu, dtype, form):
+    """Values whose plain sum of n terms of at most 1 stays in float32's range, with
+    scores that grow along the keys: no term is above 1."""
+    print("attention large values", dtype, form, flush=True)
+    rng = np.random.default_rng(5)
+    heads, group, page, news, lens, _ = FORMS[form]
+    dh, t = 64, getattr(gpu, dtype)
+    c, table = form_cache(gpu, rng, form, dh, lambda rng, shape: (
+        np.full(shape, 2), np.full(shape[:-1] + (2,), 127)))
+    power = 127 - 3 - math.ceil(math.log2(max(lens)))        # 6 2^power, the longest sequence's times: below 2^127
+    c.v_scales.fill_(127 + power)
+    c.v_codes.bitwise_and_(0x33).bitwise_or_(0x44)           # 2 to 6, none negative
+    code = np.full(c.k_codes.shape[:3] + (dh,), 2)           # 1.0
+    for b, n in enumerate(lens):
+        for j in range(n):                                   # 5.4 powers of two more every 32 keys, ...
+            code[table[b][j // page], :, j % page, :j // 32 % 12] = 6        # ... 4.0 in place of 1.0
+    c.k_codes.copy_(gpu.from_numpy((code[..., 0::2] | code[..., 1::2] << 4).astype(np.uint8)))
+    q = gpu.full((sum(news), heads * group, dh), 1.25, device="cuda").to(t)
+    kept = 2.0 ** -23 if dtype == "float32" else 2.0 ** -16
+    for name, y, lse, qd, k, v, _ in run_form(gpu, c, form, table, q, 1.0):
+        z = k @ qd
+        p = np.exp(z - z.max())
+        want, d, tol = mean_of_values(p, 2.0 ** -22 * (1 + np.abs(z - z.max())), v, kept)
+        close(y, want, tol + half_step(gpu, t, want) * 1.001, name)
+        ref = z.max() + np.log(p.sum())
+        close(np.array(lse), np.array(ref), 2.0 ** -22 * abs(ref) + 2.0 ** -21 + d, name + " lse")
