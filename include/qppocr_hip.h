@@ -408,7 +408,7 @@ typedef struct {
   const int32_t* lens;        /* [batch] */
   const int32_t* starts;      /* [batch + 1], not decreasing, or NULL */
   int32_t dtype, heads, max_new, max_len;
-  float scale;                /* finite, not 0 */
+  float scale;                /* 1.18e-38 to 2.35e38 in magnitude */
   int32_t causal, window;     /* window 0: none */
   void* workspace;
   size_t workspace_bytes;

@@ -789,8 +789,9 @@ static int attn4_check(const qph_cache4* c, const qph_attn4* p, int* shift) {
   if (p->heads <= 0 || p->heads % c->heads)
     return fail(QPH_EINVAL, "attention_cache4: query heads are no multiple of the cache's heads");
   if (p->heads > 65536) return fail(QPH_EUNSUPPORTED, "attention_cache4: more than 65536 query heads");
-  if (!std::isfinite(p->scale) || p->scale == 0.0f)
-    return fail(QPH_EINVAL, "attention_cache4: scale is zero or not finite");
+  // (device code takes subnormal numbers as zeros, and uses scale log2 e)
+  if (!std::isnormal(p->scale) || !std::isfinite(p->scale * kLog2e))
+    return fail(QPH_EINVAL, "attention_cache4: scale is zero, subnormal or too large");
   if (p->batch > INT32_MAX / c->heads || p->max_pages > INT32_MAX)
     return fail(QPH_EUNSUPPORTED, "attention_cache4: more than 2^31 - 1 sequences' heads or pages");
   if (!p->starts && p->batch && p->tokens != p->batch * (int64_t)p->max_new)

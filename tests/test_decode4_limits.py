@@ -1,0 +1,17 @@
+"""Limits of the 4-bit operators' C calls, on the host: what a call may ask for
+and still be launched, and what is refused (no GPU, no context)."""
+import ctypes
+
+import pytest
+
+from test_decode4_host import A, EINVAL, EUNSUPPORTED, attn, cache, lib, refused  # noqa: F401
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("bad,good", [(1e-45, 1.18e-38), (1.17e-38, 1.18e-38), (2.36e38, 2.35e38), (3.4e38, 2.35e38)])
+def test_smallest_and_largest_scale(lib, sign, bad, good):  # noqa: F811
+    """The device's arithmetic takes a subnormal scale as zero, and multiplies
+    scores by scale log2 e."""
+    for scale, text in ((bad, "scale"), (good, "null context")):
+        a = attn(scale=sign * scale)
+        refused(lib, lib.qph_attention_cache4(None, ctypes.byref(cache()), ctypes.byref(a)), EINVAL, text)
