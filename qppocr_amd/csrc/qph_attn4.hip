@@ -722,7 +722,11 @@ static Attn4Plan attn4_plan(const qph_cache4* c, const qph_attn4* p) {
   r.nq = many ? 2 : 1;
   r.ws = many ? 1 : 4;
   const int64_t tiles = (rows + 16 * r.nq - 1) / (16 * r.nq);
-  r.row_tiles = (int)std::min<int64_t>(std::max<int64_t>(1, r.ws == 4 ? tiles : (tiles + 3) / 4), 1 << 20);
+  // max_new is a bound for every sequence, and one long prompt among single tokens
+  // leaves most of the workgroups that it would make empty: past a million in all
+  // (some rounds of the card, whatever their work) they take further tiles in turn.
+  r.row_tiles = (int)std::clamp<int64_t>(r.ws == 4 ? tiles : (tiles + 3) / 4, 1,
+                                         std::max<int64_t>(1, ((int64_t)1 << 20) / seqs));
   r.splits = 1;
   r.chunk = (int64_t)1 << 40;
   const int64_t blocks = r.row_tiles * seqs;
@@ -830,7 +834,7 @@ QPH_API int qph_attention_cache4(qph_ctx* ctx, const qph_cache4* cache, const qp
                                 " bytes, needs " + std::to_string(p.workspace));
   if ((uintptr_t)args->workspace % 16)
     return fail(QPH_EINVAL, "attention_cache4: workspace is not 16-byte aligned");
-  if ((int64_t)p.row_tiles * p.splits * cache->heads * args->batch > INT32_MAX)
+  if ((int64_t)p.row_tiles * p.splits * cache->heads * args->batch > kMaxGroups)
     return fail(QPH_EUNSUPPORTED, "attention_cache4: batch too large for one call");
   if (!ctx) return fail(QPH_EINVAL, "null context");
   if (none) return QPH_OK;

@@ -30,6 +30,10 @@ struct F32 { typedef float type; static constexpr int terms = 3; };
 struct F16 { typedef _Float16 type; static constexpr int terms = 2; };
 struct BF16 { typedef __bf16 type; static constexpr int terms = 1; };
 
+// Workgroups of 256 threads along an axis of a launch, which HIP allows less
+// than 2^32 threads.
+constexpr int64_t kMaxGroups = (1 << 24) - 1;
+
 inline bool dtype_valid(int32_t d) { return d == QPH_F32 || d == QPH_F16 || d == QPH_BF16; }
 
 // Makes the context's device current for one call and puts the caller's back.

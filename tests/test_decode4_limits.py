@@ -15,3 +15,13 @@ def test_smallest_and_largest_scale(lib, sign, bad, good):  # noqa: F811
     for scale, text in ((bad, "scale"), (good, "null context")):
         a = attn(scale=sign * scale)
         refused(lib, lib.qph_attention_cache4(None, ctypes.byref(cache()), ctypes.byref(a)), EINVAL, text)
+
+
+def test_most_sequences_of_an_attention(lib):  # noqa: F811
+    """Workgroups: one at least a sequence and cache head; bounds on new tokens and
+    keys make no more of them than can be launched."""
+    c = cache(heads=8)
+    for batch, code, text in (((1 << 21) - 1, EINVAL, "null context"), (1 << 21, EUNSUPPORTED, "batch too large")):
+        for new in (1, 5000, (1 << 31) - 1):
+            a = attn(batch=batch, heads=32, max_new=new, max_len=(1 << 31) - 1)
+            refused(lib, lib.qph_attention_cache4(None, ctypes.byref(c), ctypes.byref(a)), code, text)

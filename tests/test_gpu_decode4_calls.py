@@ -6,7 +6,8 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_decode4 import DTYPES, close, half_step, host, make_cache, numbers, tables
+from test_gpu_decode4 import (DTYPES, attend_row, close, half_step, host, make_cache, numbers,
+                              tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -240,3 +241,34 @@ def test_attention_values_near_the_largest_number(gpu, dtype, form):
         close(y, want, tol + half_step(gpu, t, want) * 1.001, name)
         ref = z.max() + np.log(p.sum())
         close(np.array(lse), np.array(ref), 2.0 ** -22 * abs(ref) + 2.0 ** -21 + d, name + " lse")
+
+
+@pytest.mark.parametrize("dh,group,bound", [(256, 4, 1 << 17), (64, 2, 1 << 17), (64, 16, 1 << 20)])
+def test_attention_bounds_far_past_the_new_tokens(gpu, dh, group, bound):
+    """64 sequences of a few new tokens under a bound as one long prompt among them
+    would need it (once 2^24 workgroups and more, which cannot be launched)."""
+    print("attention bound", dh, group, bound, flush=True)
+    rng = np.random.default_rng(dh)
+    page, heads = 32, 8
+    lens = [int(x) for x in rng.integers(1, 50, 64)]
+    news = [int(x) for x in rng.integers(0, 4, 64)]
+    news[5], lens[5] = 40, 60
+    pages = sum((n + page - 1) // page for n in lens) + 1
+    c = make_cache(gpu, rng, pages, page, heads, dh)
+    table = tables(rng, pages, page, lens)
+    st = [0] + list(np.cumsum(news))
+    i32 = dict(dtype=gpu.int32, device="cuda")
+    q = gpu.from_numpy(rng.standard_normal((st[-1], heads * group, dh)).astype(np.float32)).cuda().bfloat16()
+    from qppocr_amd import ops
+    args = q, c, gpu.tensor(table, **i32), gpu.tensor(lens, **i32), dh ** -0.5
+    y, s = ops.attention_cache4(*args, starts=gpu.tensor(st, **i32), max_new=bound, lse=True)
+    y, s, qd = host(y), host(s), host(q)
+    k, v = numbers(c)
+    for b in (0, 5, 6, 20, 63):
+        for i in range(news[b]):
+            pos = np.arange(max(0, lens[b] - news[b] + i + 1))
+            pg = np.array(table[b])[pos // page]
+            want, tol, (lse, ltol) = attend_row(qd[st[b] + i], k[pg, pos % page], v[pg, pos % page],
+                                                dh ** -0.5, 1, group)
+            close(y[st[b] + i], want, tol + half_step(gpu, q.dtype, want) * 1.001, f"token {b} {i}")
+            close(s[st[b] + i], lse, ltol, f"lse of token {b} {i}")
