@@ -655,30 +655,30 @@ static int cache4_io(qph_ctx* ctx, const qph_cache4* c, void* k, void* v, int32_
   if (!dtype_valid(dtype)) return fail(QPH_EINVAL, w + ": unknown element type");
   if (tokens < 0) return fail(QPH_EINVAL, w + ": negative token count");
   if (tokens && (!k || !v || !slots || !ks || !vs)) return fail(QPH_EINVAL, w + ": NULL argument");
-  if (!ctx) return fail(QPH_EINVAL, "null context");
-  if (tokens == 0) return QPH_OK;
   Cache4Io a{};
-  a.kc = (unsigned char*)c->k_codes; a.ks = (unsigned char*)c->k_scales;
-  a.vc = (unsigned char*)c->v_codes; a.vs = (unsigned char*)c->v_scales;
-  a.slots_n = c->n_pages << shift;
-  a.shift = shift;
   a.heads = (unsigned)c->heads;
   a.words = (unsigned)c->dh / 8;
-  a.slots = slots;
-  a.tokens = tokens;
-  a.k = k; a.v = v;
-  a.kt = ks[0]; a.kh = ks[1]; a.vt = vs[0]; a.vh = vs[1];
   const unsigned units = a.heads * a.words;
   a.per = (int)std::max(1u, 256u / units);
   // Tokens in flight a thread: four where workgroups are many (reading 65521
   // tokens of 8 x 128: 69 us, 94 with one and 67 with eight; 300000 of 1 x 64:
   // 18, 20 and 21), one where they are few.
   const int flight = tokens / a.per >= 8192 ? 4 : 1;
-  const int64_t groups = (tokens + a.per * flight - 1) / (a.per * flight);
-  if (groups > INT32_MAX) return fail(QPH_EUNSUPPORTED, w + ": too many tokens for one call");
+  if (tokens > kMaxGroups * a.per * flight)
+    return fail(QPH_EUNSUPPORTED, w + ": too many tokens for one call");
+  if (!ctx) return fail(QPH_EINVAL, "null context");
+  if (tokens == 0) return QPH_OK;
+  a.kc = (unsigned char*)c->k_codes; a.ks = (unsigned char*)c->k_scales;
+  a.vc = (unsigned char*)c->v_codes; a.vs = (unsigned char*)c->v_scales;
+  a.slots_n = c->n_pages << shift;
+  a.shift = shift;
+  a.slots = slots;
+  a.tokens = tokens;
+  a.k = k; a.v = v;
+  a.kt = ks[0]; a.kh = ks[1]; a.vt = vs[0]; a.vh = vs[1];
   OnDevice dev(ctx);
   QPH_TRY(dev.rc());
-  const dim3 grid((unsigned)groups, 2);
+  const dim3 grid(ceil_div(tokens, a.per * flight), 2);
 #define QPH_LAUNCH(E)                                                                              \
   do {                                                                                             \
     auto fn = write ? (flight == 4 ? cache4_write_kernel<E, 4> : cache4_write_kernel<E, 1>)        \
@@ -712,7 +712,7 @@ QPH_API int qph_quantize4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t ro
   if (k > (1 << 30)) return fail(QPH_EUNSUPPORTED, "quantize4: more than 2^30 columns");
   if (rows && (!x || !codes || !scales)) return fail(QPH_EINVAL, "quantize4: NULL argument");
   if ((uintptr_t)codes % 16) return fail(QPH_EINVAL, "quantize4: codes are not 16-byte aligned");
-  if (rows > ((int64_t)INT32_MAX * 256) / ((k + 127) / 128 * 4))
+  if (rows > kMaxGroups * 256 / ((k + 127) / 128 * 4))
     return fail(QPH_EUNSUPPORTED, "quantize4: too many blocks for one call");
   if (!ctx) return fail(QPH_EINVAL, "null context");
   if (rows == 0) return QPH_OK;
@@ -738,9 +738,10 @@ QPH_API int qph_linear4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t x_st
   if (rows && (!x || !codes || !scales || !y)) return fail(QPH_EINVAL, "linear4: NULL argument");
   if ((uintptr_t)codes % 16 || (uintptr_t)scales % 4)
     return fail(QPH_EINVAL, "linear4: codes are not 16-byte or scales not 4-byte aligned");
-  // columns, rows and k are counted in 32 bits, row tiles by the grid's second axis
-  if (n > (1 << 30) || k > (1 << 30) || rows > 65535 * 16)
-    return fail(QPH_EUNSUPPORTED, "linear4: more than 2^30 columns or inputs, or 1048560 rows");
+  // columns, rows and k are counted in 32 bits, row tiles by the grid's second axis;
+  // 512 threads take 48 columns or more where there are many
+  if (n > (1 << 28) || k > (1 << 30) || rows > 65535 * 16)
+    return fail(QPH_EUNSUPPORTED, "linear4: more than 2^28 columns, 2^30 inputs or 1048560 rows");
   if (!ctx) return fail(QPH_EINVAL, "null context");
   if (rows == 0) return QPH_OK;
   Lin4 a{};

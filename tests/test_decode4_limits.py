@@ -17,6 +17,29 @@ def test_smallest_and_largest_scale(lib, sign, bad, good):  # noqa: F811
         refused(lib, lib.qph_attention_cache4(None, ctypes.byref(cache()), ctypes.byref(a)), EINVAL, text)
 
 
+def test_most_tokens_of_a_cache_call(lib):  # noqa: F811
+    """A launch has fewer than 2^32 threads along an axis: 2^24 - 1 workgroups."""
+    st = (ctypes.c_int64 * 2)(0, 0)
+    for fn in (lib.qph_cache4_write, lib.qph_cache4_read):
+        for heads, dh, most in ((64, 256, 4 * ((1 << 24) - 1)), (1, 32, 4 * 64 * ((1 << 24) - 1))):
+            c = cache(heads=heads, dh=dh)
+            for tokens, code, text in ((most, EINVAL, "null context"), (most + 1, EUNSUPPORTED, "too many tokens")):
+                refused(lib, fn(None, ctypes.byref(c), A, A, 0, tokens, st, st, A), code, text)
+
+
+def test_most_blocks_of_a_weight(lib):  # noqa: F811
+    for k, groups in ((128, 4), (1 << 20, 1 << 15)):
+        rows = ((1 << 24) - 1) * 256 // groups
+        for n, code, text in ((rows, EINVAL, "null context"), (rows + 1, EUNSUPPORTED, "blocks")):
+            refused(lib, lib.qph_quantize4(None, A, 1, n, k, 0, 1, A, A), code, text)
+
+
+def test_most_columns_of_a_linear(lib):  # noqa: F811
+    for rows in (1, 40, 3000):
+        for n, code, text in ((1 << 28, EINVAL, "null context"), ((1 << 28) + 1, EUNSUPPORTED, "2^28 columns")):
+            refused(lib, lib.qph_linear4(None, A, 0, 64, A, A, None, rows, 64, n, None, None, A), code, text)
+
+
 def test_most_sequences_of_an_attention(lib):  # noqa: F811
     """Workgroups: one at least a sequence and cache head; bounds on new tokens and
     keys make no more of them than can be launched."""
