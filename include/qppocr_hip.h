@@ -41,7 +41,8 @@ extern "C" {
 typedef struct qph_ctx qph_ctx;
 
 /* Device context + stream: the DeviceContext analogue
- * (qppocr-core/src/device.rs:83-101).  device = HIP device ordinal. */
+ * (qppocr-core/src/device.rs:83-101).  device = HIP device ordinal, which
+ * becomes the calling thread's current device. */
 QPH_API int qph_ctx_create(int device, qph_ctx** out);
 QPH_API int qph_ctx_destroy(qph_ctx* ctx);
 /* Use an external HIP stream (e.g. a framework's current stream) instead of

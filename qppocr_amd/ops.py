@@ -481,7 +481,8 @@ def _enqueue(device, fn, *args):
     with _queue_lock:
         entry = _queued.get(device)
         if entry is None:
-            entry = _queued[device] = [new_context(device), None]
+            with torch.cuda.device(device):      # (which puts the caller's device back)
+                entry = _queued[device] = [new_context(device), None]
         if entry[1] != stream:
             check(_lib.load().qph_ctx_set_stream(entry[0], stream))
             entry[1] = stream

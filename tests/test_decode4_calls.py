@@ -63,3 +63,34 @@ def test_every_buffer_has_its_own_type(calls, default, dtype):
         assert ops.linear4(torch.zeros((2, 64), dtype=dtype), w).dtype == dtype
     finally:
         torch.set_default_dtype(was)
+
+
+def test_first_call_leaves_the_callers_device(monkeypatch):
+    """The context that a device's first call makes leaves the thread's device as it was."""
+    now, log = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.was, now[0] = now[0], self.index
+
+        def __exit__(self, *a):
+            now[0] = self.was
+
+    class Library:
+        def qph_ctx_create(self, device, out):
+            now[0] = device                # as the library does
+            return 0
+
+        def qph_ctx_set_stream(self, ctx, stream):
+            return 0
+    monkeypatch.setattr(ops, "_queued", {})
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 64)
+    monkeypatch.setattr(_lib, "load", lambda: Library())
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for device in (3, 3, 0, 1):
+        ops._enqueue(device, lambda ctx, *a: log.append(a) or 0, "x")
+        assert now[0] == 0
+    assert log == [("x",)] * 4 and sorted(ops._queued) == [0, 1, 3]
