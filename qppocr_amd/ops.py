@@ -514,11 +514,36 @@ def _plain(what, name, t, dtype, shape, device):
     _on(what, device, name, t)
 
 
-class Weight4:
+class _Fixed:
+    """What its __init__ sets stays: the calls use addresses taken then.  A copy of
+    any kind is made by __init__ again, from what _parts names."""
+    _names = frozenset()
+    _parts = ()
+
+    def __setattr__(self, name, value):
+        if name in self._names:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed; make another one")
+        self.__dict__[name] = value
+
+    def __delattr__(self, name):
+        if name in self._names:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed")
+        object.__delattr__(self, name)
+
+    def __reduce__(self):
+        return type(self), tuple(getattr(self, name) for name in self._parts)
+
+    def _fix(self, **names):
+        self.__dict__.update(names, _names=frozenset(names) | {"_names"})
+
+
+class Weight4(_Fixed):
     """A linear's weight [n, k] in 4 bits (the format: include/qppocr_hip.h):
     codes uint8 [n, kp / 2] and scales uint8 [n, kp / 32], kp = k rounded up to
     128, elements past k zero.  quantize4 makes one; a caller may bring the
-    two tensors."""
+    two tensors, whose memory it is then made of (their contents may change, the
+    tensors may not be replaced or moved)."""
+    _parts = "codes", "scales", "k"
 
     def __init__(self, codes, scales, k):
         if codes.dim() != 2 or k <= 0:
@@ -528,9 +553,8 @@ class Weight4:
         _plain("Weight4", "scales", scales, torch.uint8, (n, kp // 32), codes.device)
         if codes.data_ptr() % 16 or scales.data_ptr() % 4:
             raise ValueError("Weight4: codes are not 16-byte or scales not 4-byte aligned")
-        self.codes, self.scales, self.n, self.k = codes, scales, n, int(k)
-        self.device, self._index = codes.device, codes.device.index
-        self._ptrs = codes.data_ptr(), scales.data_ptr()
+        self._fix(codes=codes, scales=scales, n=n, k=int(k), device=codes.device,
+                  _index=codes.device.index, _ptrs=(codes.data_ptr(), scales.data_ptr()))
 
 
 def quantize4(w):
@@ -582,11 +606,12 @@ def linear4(x, w, bias=None, act_kind=ACT_NONE, residual=None):
     return y
 
 
-class Cache4:
+class Cache4(_Fixed):
     """A paged cache of keys and values in 4 bits (the format and layout:
     include/qppocr_hip.h): codes uint8 [pages, heads, page size, dh / 2] and
     scales uint8 [pages, heads, page size, dh / 32] of either.  cache4 makes
-    an empty one."""
+    an empty one; a caller may bring the four tensors, as for a Weight4."""
+    _parts = "k_codes", "k_scales", "v_codes", "v_scales"
 
     def __init__(self, k_codes, k_scales, v_codes, v_scales):
         if k_codes.dim() != 4:
@@ -602,13 +627,11 @@ class Cache4:
                               ("k_scales", k_scales, half // 16),
                               ("v_scales", v_scales, half // 16)):
             _plain("Cache4", name, t, torch.uint8, (pages, heads, page, last), k_codes.device)
-        self.k_codes, self.k_scales = k_codes, k_scales
-        self.v_codes, self.v_scales = v_codes, v_scales
-        self.pages, self.heads, self.page_size, self.dh = pages, heads, page, 2 * half
-        self.device, self._index = k_codes.device, k_codes.device.index
-        self._c = _lib.Cache4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-                              v_scales.data_ptr(), pages, page, heads, 2 * half)
-        self._ref = ctypes.byref(self._c)
+        c = _lib.Cache4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                        v_scales.data_ptr(), pages, page, heads, 2 * half)
+        self._fix(k_codes=k_codes, k_scales=k_scales, v_codes=v_codes, v_scales=v_scales,
+                  pages=pages, heads=heads, page_size=page, dh=2 * half, device=k_codes.device,
+                  _index=k_codes.device.index, _c=c, _ref=ctypes.byref(c))
 
 
 def cache4(pages, page_size, heads, dh, device="cuda"):

@@ -1,7 +1,9 @@
 """The Python calls of the 4-bit operators as the library gets them, on the host:
 the device's check and the library's call are replaced, the tensors are host
 tensors, and nothing is computed."""
+import copy
 import os
+import pickle
 
 import pytest
 import torch
@@ -94,3 +96,42 @@ def test_first_call_leaves_the_callers_device(monkeypatch):
         ops._enqueue(device, lambda ctx, *a: log.append(a) or 0, "x")
         assert now[0] == 0
     assert log == [("x",)] * 4 and sorted(ops._queued) == [0, 1, 3]
+
+
+@pytest.mark.parametrize("name", ["codes", "scales", "n", "k", "device"])
+def test_a_weights_memory_is_fixed(calls, name):
+    """A call reads the memory a Weight4 was made of, so another tensor in its place
+    is refused rather than not looked at."""
+    w = ops.quantize4(torch.zeros((100, 8)))
+    with pytest.raises(AttributeError, match=name):
+        setattr(w, name, getattr(w, name))
+    with pytest.raises(AttributeError, match=name):
+        delattr(w, name)
+    w.note = "mine"
+    w.note = "other"
+    ops.linear4(torch.zeros((2, 100)), w)
+    assert calls[-1][2][3:5] == (w.codes.data_ptr(), w.scales.data_ptr())
+
+
+@pytest.mark.parametrize("name", ["k_codes", "k_scales", "v_codes", "v_scales", "pages", "heads",
+                                  "page_size", "dh", "device"])
+def test_a_caches_memory_is_fixed(calls, name):
+    c = cache()
+    with pytest.raises(AttributeError, match=name):
+        setattr(c, name, getattr(c, name))
+    with pytest.raises(AttributeError, match=name):
+        delattr(c, name)
+    assert c._c.k_codes == c.k_codes.data_ptr() and c._c.v_scales == c.v_scales.data_ptr()
+
+
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))], ids=["deepcopy", "pickle"])
+def test_copies_have_their_own_memory(calls, how):
+    w, c = ops.quantize4(torch.zeros((100, 8))), cache()
+    w2, c2 = how(w), how(c)
+    assert (w2.n, w2.k, w2.device) == (w.n, w.k, w.device) and w2.codes.data_ptr() != w.codes.data_ptr()
+    assert w2._ptrs == (w2.codes.data_ptr(), w2.scales.data_ptr())
+    assert (c2.pages, c2.heads, c2.page_size, c2.dh) == (c.pages, c.heads, c.page_size, c.dh)
+    assert c2._c.k_codes == c2.k_codes.data_ptr() != c.k_codes.data_ptr()
+    assert c2._c.v_scales == c2.v_scales.data_ptr() != c.v_scales.data_ptr()
+    w3 = copy.copy(w)
+    assert w3._ptrs == w._ptrs
