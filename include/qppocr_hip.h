@@ -388,7 +388,8 @@ QPH_API int qph_cache4_read(qph_ctx* ctx, const qph_cache4* cache, void* k, void
  *   out = sum_j softmax_j(scale q . k_j) v_j
  *   lse = log sum_j exp(scale q . k_j)     (float32 [tokens][heads], or NULL)
  * A row that sees no key gets zeros and -infinity.  Rows that no sequence has
- * are left as they were.  max_new and max_len (host) bound the sequences' new
+ * are left as they were.  out may be q itself (with its strides); its elements
+ * share no memory with q's otherwise, nor with each other.  max_new and max_len (host) bound the sequences' new
  * and cached tokens; they choose the work's split, and longer ones only run
  * slower.  lens are cut at max_pages pages.  Scores, sums and the running
  * maximum are float32 (scores of any finite size; one past float32's range

@@ -654,6 +654,38 @@ def _rows4(what, name, t, cache, tokens, heads):
     return strides[:2]
 
 
+def _reach(dims):
+    """The last element's offset of dims (stride, size), or None where two elements may
+    have one place (each stride must pass all that the smaller ones reach)."""
+    last = 0
+    for stride, size in sorted(dims):
+        if size > 1:
+            if stride <= last:
+                return None
+            last += stride * (size - 1)
+    return last
+
+
+def _writable(what, name, t, other=None, other_name=None):
+    """Refuses an output whose elements share memory, among themselves or with `other`."""
+    if not t.numel():
+        return
+    dims = list(zip(t.stride(), t.shape))
+    reach = _reach(dims)
+    if reach is None:
+        raise ValueError(f"{what}: {name} of strides {t.stride()} overlaps itself")
+    if other is None or not other.numel():
+        return
+    # apart from end to end, or of one layout whose two copies interleave
+    size, delta = t.element_size(), other.data_ptr() - t.data_ptr()
+    length = other.element_size() * (1 + sum(st * (n - 1) for st, n in zip(other.stride(), other.shape)))
+    if delta >= (reach + 1) * size or -delta >= length:
+        return
+    if delta % size or (t.stride(), t.shape, t.dtype) != (other.stride(), other.shape, other.dtype) or \
+            _reach(dims + [(abs(delta) // size, 2)]) is None:
+        raise ValueError(f"{what}: {name} and {other_name} share memory")
+
+
 def cache4_write(cache, k, v, slots):
     """Quantises tokens' keys and values [tokens, heads, dh] (tokens and heads
     of any strides) into their slots, int64 [tokens]: page * page_size + place.
@@ -688,6 +720,9 @@ def cache4_read(cache, slots, dtype=torch.float32, out=None):
         raise ValueError("cache4_read: k and v of one type")
     ks = _rows4("cache4_read", "k", k, cache, n, cache.heads)
     vs = _rows4("cache4_read", "v", v, cache, n, cache.heads)
+    if out is not None:
+        _writable("cache4_read", "k", k, v, "v")
+        _writable("cache4_read", "v", v)
     _plain("cache4_read", "slots", slots, torch.int64, (n,), cache.device)
     _enqueue(cache._index, _lib.load().qph_cache4_read, cache._ref, k.data_ptr(), v.data_ptr(), d, n,
              _dims(ks), _dims(vs), slots.data_ptr())
@@ -717,7 +752,8 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
     pages and cached tokens, its new ones the last of them.  starts int32
     [batch + 1]: sequence b's new tokens are q[starts[b]:starts[b + 1]], at most
     max_new (needed then); without starts every sequence has tokens / batch.
-    max_len bounds lens (default: all of the table's pages).  causal hides
+    max_len bounds lens (default: all of the table's pages).  out may be q itself, and
+    shares no memory with it otherwise.  causal hides
     later keys, window > 0 all but the last `window` up to a token's own.  A
     row that sees no key is zero; rows of no sequence keep what out holds.
     Returns out, or (out, lse) with the sums' logarithms, float32 [tokens,
@@ -752,11 +788,15 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
         max_new = each
     if max_len is None:
         max_len = min(pages * cache.page_size, 0x7fffff00)
-    if out is None:
+    own = out is None
+    if own:
         out = q.new_empty((tokens, heads, dh))
     elif out.dtype != q.dtype:
         raise ValueError(f"{what}: out is {out.dtype}, q {q.dtype}")
     os = _rows4(what, "out", out, cache, tokens, heads)
+    if not own:
+        same = out.data_ptr() == q.data_ptr() and os == qs
+        _writable(what, "out", out, None if same else q, "q")
     sums = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if lse else None
     max_new, max_len, window, causal = int(max_new), int(max_len), int(window), int(bool(causal))
     size = _workspace4(cache.pages, cache.page_size, cache.heads, dh, d, heads, tokens, batch, pages,

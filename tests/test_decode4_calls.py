@@ -135,3 +135,57 @@ def test_copies_have_their_own_memory(calls, how):
     assert c2._c.v_scales == c2.v_scales.data_ptr() != c.v_scales.data_ptr()
     w3 = copy.copy(w)
     assert w3._ptrs == w._ptrs
+
+
+def views(dtype=torch.float32):
+    """(k, v, the pair does not overlap) of 5 tokens, 2 heads of 64."""
+    z = torch.zeros
+    both = z((5, 2, 2, 64), dtype=dtype)
+    packed = z((5, 7, 64), dtype=dtype)
+    long = z(5 * 2 * 2 * 64 + 640, dtype=dtype)
+
+    def at(offset, *strides):
+        return long.as_strided((5, 2, 64), strides + (1,), offset)
+    yield both[:, 0], both[:, 1], True
+    yield both[:, 1], both[:, 0], True
+    yield both[:, :, 0], both[:, :, 1], True
+    yield packed[:, 1:3], packed[:, 4:6], True
+    yield packed[:, 4:6], packed[:, 2:4], True
+    yield z((5, 2, 64), dtype=dtype), z((2, 5, 64), dtype=dtype).transpose(0, 1), True
+    yield at(0, 128, 64), at(640, 64, 320), True
+    yield packed[:, 1:3], packed[:, 2:4], False
+    yield both[:, 0], both[:, 0], False
+    yield at(0, 128, 64), at(64, 128, 64), False
+    yield at(0, 128, 64), at(639, 64, 320), False
+    yield z((1, 2, 64), dtype=dtype).expand(5, 2, 64), z((5, 2, 64), dtype=dtype), False
+    yield z((5, 2, 64), dtype=dtype), z((5, 1, 64), dtype=dtype).expand(5, 2, 64), False
+    yield at(0, 100, 64), at(1000, 128, 64), False
+    yield at(0, 128, 63), at(1000, 128, 64), False
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("i", range(15))
+def test_outputs_that_overlap(calls, dtype, i):
+    k, v, good = list(views(dtype))[i]
+    slots = torch.zeros(5, dtype=torch.int64)
+    if good:
+        assert ops.cache4_read(cache(), slots, out=(k, v)) == (k, v)
+        assert attend(cache(), 5, 2, dtype, q=k, out=v) is v
+    else:
+        with pytest.raises(ValueError, match="overlaps itself|share memory"):
+            ops.cache4_read(cache(), slots, out=(k, v))
+        if k.data_ptr() != v.data_ptr():           # (out may be q itself)
+            # v as out, and k where only that overlaps itself
+            q, out = (v, k) if k.stride() in ((0, 64, 1), (100, 64, 1), (128, 63, 1)) else (k, v)
+            with pytest.raises(ValueError, match="overlaps itself|share memory"):
+                attend(cache(), 5, 2, dtype, q=q, out=out)
+
+
+def test_an_output_that_is_the_query(calls):
+    q = torch.zeros((5, 2, 64))
+    assert attend(cache(), 5, 2, q=q, out=q) is q
+    # one token, or one head: nothing of theirs can overlap, whatever the stride says
+    one = torch.zeros((1, 2, 64))
+    attend(cache(), 1, 2, q=one, out=torch.zeros(128).as_strided((1, 2, 64), (0, 64, 1)))
+    none = torch.zeros((0, 2, 64))
+    ops.cache4_read(cache(), torch.zeros(0, dtype=torch.int64), out=(none, none))

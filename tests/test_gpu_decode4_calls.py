@@ -272,3 +272,27 @@ def test_attention_bounds_far_past_the_new_tokens(gpu, dh, group, bound):
                                                 dh ** -0.5, 1, group)
             close(y[st[b] + i], want, tol + half_step(gpu, q.dtype, want) * 1.001, f"token {b} {i}")
             close(s[st[b] + i], lse, ltol, f"lse of token {b} {i}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", list(FORMS))
+def test_attention_in_place(gpu, dtype, form):
+    """out may be q itself, packed among other rows: the same bits as apart from it."""
+    from qppocr_amd import ops
+    print("attention in place", dtype, form, flush=True)
+    rng = np.random.default_rng(41)
+    heads, group, page, news, lens, _ = FORMS[form]
+    dh = 64
+    c = make_cache(gpu, rng, sum((n + page - 1) // page for n in lens) + 1, page, heads, dh)
+    table = tables(rng, c.pages, page, lens)
+    st, i32 = [0] + list(np.cumsum(news)), dict(dtype=gpu.int32, device="cuda")
+    packed = gpu.from_numpy(rng.standard_normal((st[-1], heads * group + 3, dh)).astype(np.float32))
+    packed = packed.cuda().to(getattr(gpu, dtype))
+    kept = packed.clone()
+    q = packed[:, 2:2 + heads * group]
+    args = c, gpu.tensor(table, **i32), gpu.tensor(lens, **i32), 0.125
+    kw = dict(starts=gpu.tensor(st, **i32), max_new=max(news), max_len=max(lens))
+    want = ops.attention_cache4(q, *args, **kw)
+    assert ops.attention_cache4(q, *args, out=q, **kw) is q
+    assert (host(q) == host(want)).all()
+    assert (packed[:, :2] == kept[:, :2]).all() and (packed[:, 2 + heads * group:] == kept[:, 2 + heads * group:]).all()
