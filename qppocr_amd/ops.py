@@ -12,7 +12,8 @@ are synchronous with respect to torch's current stream: the stream is drained
 before the library's own stream runs the kernel, and the library stream is
 drained before returning.  The 4-bit operators do not wait: they are enqueued on
 torch's current stream of the tensors' device, in its order, and may be captured
-into a graph.  Errors raise QphError (no silent fallback).
+into a graph; they compute no gradients and refuse tensors that require one.
+Errors raise QphError (no silent fallback).
 """
 import ctypes
 import functools
@@ -514,6 +515,15 @@ def _plain(what, name, t, dtype, shape, device):
     _on(what, device, name, t)
 
 
+def _no_grad(what, *tensors):
+    """Refuses tensors whose gradient the call would drop without a word."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what}: no gradient is computed, but a tensor requires one (detach "
+                                 "it, or call under torch.no_grad())")
+
+
 class _Fixed:
     """What its __init__ sets stays: the calls use addresses taken then.  A copy of
     any kind is made by __init__ again, from what _parts names."""
@@ -584,6 +594,7 @@ def linear4(x, w, bias=None, act_kind=ACT_NONE, residual=None):
     if x.dim() < 1 or x.shape[-1] != k:
         raise ValueError(f"linear4: x {tuple(x.shape)} against a weight of {k} inputs")
     _on("linear4", w.device, "x", x)
+    _no_grad("linear4", x, bias, residual)
     if x.dim() == 2:
         rows, x2 = x.shape[0], x
         y = x.new_empty((rows, n))
@@ -698,6 +709,7 @@ def cache4_write(cache, k, v, slots):
     ks = _rows4("cache4_write", "k", k, cache, n, cache.heads)
     vs = _rows4("cache4_write", "v", v, cache, n, cache.heads)
     _plain("cache4_write", "slots", slots, torch.int64, (n,), cache.device)
+    _no_grad("cache4_write", k, v)
     _enqueue(cache._index, _lib.load().qph_cache4_write, cache._ref, k.data_ptr(), v.data_ptr(), d,
              n, _dims(ks), _dims(vs), slots.data_ptr())
 
@@ -721,6 +733,7 @@ def cache4_read(cache, slots, dtype=torch.float32, out=None):
     ks = _rows4("cache4_read", "k", k, cache, n, cache.heads)
     vs = _rows4("cache4_read", "v", v, cache, n, cache.heads)
     if out is not None:
+        _no_grad("cache4_read", k, v)
         _writable("cache4_read", "k", k, v, "v")
         _writable("cache4_read", "v", v)
     _plain("cache4_read", "slots", slots, torch.int64, (n,), cache.device)
@@ -766,6 +779,7 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
     tokens, heads, dh = q.shape
     dev = cache.device
     qs = _rows4(what, "q", q, cache, tokens, heads)
+    _no_grad(what, q, out)
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (
             page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError(f"{what}: page_table int32 [batch, pages], rows contiguous")

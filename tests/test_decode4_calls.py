@@ -189,3 +189,29 @@ def test_an_output_that_is_the_query(calls):
     attend(cache(), 1, 2, q=one, out=torch.zeros(128).as_strided((1, 2, 64), (0, 64, 1)))
     none = torch.zeros((0, 2, 64))
     ops.cache4_read(cache(), torch.zeros(0, dtype=torch.int64), out=(none, none))
+
+
+def test_no_gradient_is_dropped(calls):
+    """The operators compute no gradients: an input that requires one is refused while
+    gradients are recorded, and taken under no_grad; a weight to quantise is taken."""
+    p = lambda *s: torch.zeros(s, requires_grad=True)      # noqa: E731
+    z, slots = torch.zeros, torch.zeros(3, dtype=torch.int64)
+    c = cache()
+    w = ops.quantize4(p(64, 8))
+    refused = [
+        lambda: ops.linear4(p(2, 64), w), lambda: ops.linear4(z(2, 64), w, p(8)),
+        lambda: ops.linear4(z(2, 64), w, None, 0, p(2, 8)),
+        lambda: ops.linear4(p(2, 64) * 2, w),
+        lambda: ops.cache4_write(c, p(3, 2, 64), z(3, 2, 64), slots),
+        lambda: ops.cache4_write(c, z(3, 2, 64), p(3, 2, 64), slots),
+        lambda: ops.cache4_read(c, slots, out=(z(3, 2, 64), p(3, 2, 64))),
+        lambda: attend(c, q=p(3, 4, 64)), lambda: attend(c, out=p(3, 4, 64)),
+    ]
+    for call in refused:
+        n = len(calls)
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        assert len(calls) == n
+        with torch.no_grad():
+            call()
+        assert len(calls) == n + 1
