@@ -812,7 +812,10 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
         same = out.data_ptr() == q.data_ptr() and os == qs
         _writable(what, "out", out, None if same else q, "q")
     sums = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if lse else None
-    max_new, max_len, window, causal = int(max_new), int(max_len), int(window), int(bool(causal))
+    max_new, max_len, window = (min(int(n), 0x7fffffff) for n in (max_new, max_len, window))
+    if min(max_new, max_len, window) < 0:
+        raise ValueError(f"{what}: negative max_new, max_len or window")
+    causal = int(bool(causal))
     size = _workspace4(cache.pages, cache.page_size, cache.heads, dh, d, heads, tokens, batch, pages,
                        max_new, max_len, causal, window, None if at is None else 256)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None

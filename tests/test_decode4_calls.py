@@ -215,3 +215,20 @@ def test_no_gradient_is_dropped(calls):
         with torch.no_grad():
             call()
         assert len(calls) == n + 1
+
+
+def test_bounds_past_32_bits(calls):
+    """Bounds that no sequence can reach mean what they say: the widest window, the
+    longest sequences; negative ones are refused however small."""
+    starts = torch.arange(4, dtype=torch.int32)
+    top = (1 << 31) - 1
+    for big in (top, 1 << 31, (1 << 32) - 1, 1 << 32, (1 << 32) + 5, 1 << 70):
+        attend(cache(), window=big)
+        assert calls[-1][2][1]._obj.window == top
+        attend(cache(), max_len=big, max_new=big, starts=starts)
+        a = calls[-1][2][1]._obj
+        assert a.max_len == a.max_new == top and a.window == 0
+    for low in (-1, -(1 << 31) - 1, -(1 << 32), -(1 << 32) + 5):
+        for kw in (dict(window=low), dict(max_len=low), dict(max_new=low, starts=starts)):
+            with pytest.raises(ValueError, match="negative"):
+                attend(cache(), **kw)
