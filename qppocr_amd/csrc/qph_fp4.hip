@@ -64,10 +64,12 @@ __device__ __forceinline__ int64_t cache4_row(int64_t slot, int shift, unsigned 
   return ((((slot >> shift) * heads + h) << shift) + (slot & (((int64_t)1 << shift) - 1)));
 }
 
-// A word of codes (eight elements) per thread and token, U tokens (per * U a
-// workgroup) in flight; the four threads of a block of 32 share its largest
-// magnitude by two swaps inside a quad (a quad is of one token).
-template <typename E, int U>
+// A word of codes (eight elements) per thread and token; the four threads of a
+// block of 32 share its largest magnitude by two swaps inside a quad (a quad is
+// of one token).  Bound by memory; more tokens in flight a thread gain nothing,
+// the stores need no answer (four against one: 65521 tokens of 8 x 128 bfloat16
+// 83 and 75 us, 262144 334 and 301, 300000 of 1 x 64 21.3 and 20.6).
+template <typename E>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Io a) {
   const unsigned units = a.heads * a.words, total = units * (unsigned)a.per;
   const bool second = blockIdx.y != 0;
@@ -77,32 +79,26 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4Io a) {
   unsigned char* scales = second ? a.vs : a.ks;
   for (unsigned u = threadIdx.x; u < total; u += blockDim.x) {
     const unsigned lt = u / units, w = u % units, h = w / a.words, c = w % a.words;
-    const int64_t t0 = (int64_t)blockIdx.x * (a.per * U) + lt;
-    int64_t slot[U];
-    float v[U][8];
-#pragma unroll
-    for (int i = 0; i < U; i++) {
-      const int64_t t = t0 + i * a.per;
-      slot[i] = -1;
-      if (t >= a.tokens) continue;
-      slot[i] = a.slots[t];
-      load8<E>(x + t * xt + h * xh + c * 8, v[i]);
+    const int64_t t = (int64_t)blockIdx.x * a.per + lt;
+    int64_t slot = -1;
+    float v[8];
+    if (t < a.tokens) {
+      // (both at once: behind the slot's check the row would wait for it)
+      slot = a.slots[t];
+      load8<E>(x + t * xt + h * xh + c * 8, v);
     }
+    if (slot < 0 || slot >= a.slots_n) continue;
+    unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < U; i++) {
-      if (slot[i] < 0 || slot[i] >= a.slots_n) continue;
-      unsigned top = 0;
-#pragma unroll
-      for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
-      top = max(top, (unsigned)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xf, 0xf, true));  // lane ^ 1
-      top = max(top, (unsigned)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xf, 0xf, true));  // lane ^ 2
-      const int e = fp4_exponent(top);
-      const bool bad = e == -1000;
-      const int64_t row = cache4_row(slot[i], a.shift, a.heads, h);
-      ((unsigned*)codes)[row * a.words + c] =
-          bad ? 0u : fp4_encode8(v[i], scale_of_byte((unsigned)(e + 127)));
-      if (c % 4 == 0) scales[row * (a.words / 4) + c / 4] = (unsigned char)(bad ? 255 : e + 127);
-    }
+    for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    top = max(top, (unsigned)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xf, 0xf, true));  // lane ^ 1
+    top = max(top, (unsigned)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xf, 0xf, true));  // lane ^ 2
+    const int e = fp4_exponent(top);
+    const bool bad = e == -1000;
+    const int64_t row = cache4_row(slot, a.shift, a.heads, h);
+    ((unsigned*)codes)[row * a.words + c] =
+        bad ? 0u : fp4_encode8(v, scale_of_byte((unsigned)(e + 127)));
+    if (c % 4 == 0) scales[row * (a.words / 4) + c / 4] = (unsigned char)(bad ? 255 : e + 127);
   }
 }
 
@@ -655,41 +651,45 @@ static int cache4_io(qph_ctx* ctx, const qph_cache4* c, void* k, void* v, int32_
   if (!dtype_valid(dtype)) return fail(QPH_EINVAL, w + ": unknown element type");
   if (tokens < 0) return fail(QPH_EINVAL, w + ": negative token count");
   if (tokens && (!k || !v || !slots || !ks || !vs)) return fail(QPH_EINVAL, w + ": NULL argument");
-  Cache4Io a{};
-  a.heads = (unsigned)c->heads;
-  a.words = (unsigned)c->dh / 8;
-  const unsigned units = a.heads * a.words;
-  a.per = (int)std::max(1u, 256u / units);
-  // Tokens in flight a thread: four where workgroups are many (reading 65521
-  // tokens of 8 x 128: 69 us, 94 with one and 67 with eight; 300000 of 1 x 64:
-  // 18, 20 and 21), one where they are few.
-  const int flight = tokens / a.per >= 8192 ? 4 : 1;
-  if (tokens > kMaxGroups * a.per * flight)
-    return fail(QPH_EUNSUPPORTED, w + ": too many tokens for one call");
   if (!ctx) return fail(QPH_EINVAL, "null context");
   if (tokens == 0) return QPH_OK;
+  Cache4Io a{};
   a.kc = (unsigned char*)c->k_codes; a.ks = (unsigned char*)c->k_scales;
   a.vc = (unsigned char*)c->v_codes; a.vs = (unsigned char*)c->v_scales;
   a.slots_n = c->n_pages << shift;
   a.shift = shift;
-  a.slots = slots;
-  a.tokens = tokens;
-  a.k = k; a.v = v;
+  a.heads = (unsigned)c->heads;
+  a.words = (unsigned)c->dh / 8;
   a.kt = ks[0]; a.kh = ks[1]; a.vt = vs[0]; a.vh = vs[1];
+  const unsigned units = a.heads * a.words;
+  a.per = (int)std::max(1u, 256u / units);
+  // Tokens that a thread reads at once: four where workgroups are many (65521
+  // tokens of 8 x 128: 69 us, 88 with one and 67 with eight; 300000 of 1 x 64:
+  // 18.5, 19.5 and 21), one where they are few.
+  const int flight = !write && tokens / a.per >= 8192 ? 4 : 1;
   OnDevice dev(ctx);
   QPH_TRY(dev.rc());
-  const dim3 grid(ceil_div(tokens, a.per * flight), 2);
+  // (more tokens than one launch takes: in several)
+  const int64_t most = kMaxGroups * a.per * flight, size = dtype == QPH_F32 ? 4 : 2;
+  for (int64_t t = 0; t < tokens; t += most) {
+    a.tokens = std::min(most, tokens - t);
+    a.slots = slots + t;
+    a.k = (char*)k + t * ks[0] * size;
+    a.v = (char*)v + t * vs[0] * size;
+    const dim3 grid(ceil_div(a.tokens, a.per * flight), 2);
 #define QPH_LAUNCH(E)                                                                              \
   do {                                                                                             \
-    auto fn = write ? (flight == 4 ? cache4_write_kernel<E, 4> : cache4_write_kernel<E, 1>)        \
+    auto fn = write ? cache4_write_kernel<E>                                                       \
                     : (flight == 4 ? cache4_read_kernel<E, 4> : cache4_read_kernel<E, 1>);         \
     hipLaunchKernelGGL(fn, grid, dim3(256), 0, ctx->stream, a);                                    \
   } while (0)
-  if (dtype == QPH_F32) QPH_LAUNCH(F32);
-  else if (dtype == QPH_F16) QPH_LAUNCH(F16);
-  else QPH_LAUNCH(BF16);
+    if (dtype == QPH_F32) QPH_LAUNCH(F32);
+    else if (dtype == QPH_F16) QPH_LAUNCH(F16);
+    else QPH_LAUNCH(BF16);
 #undef QPH_LAUNCH
-  return launch_check(what);
+    QPH_TRY(launch_check(what));
+  }
+  return QPH_OK;
 }
 
 template <typename E>

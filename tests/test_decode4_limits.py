@@ -17,17 +17,8 @@ def test_smallest_and_largest_scale(lib, sign, bad, good):  # noqa: F811
         refused(lib, lib.qph_attention_cache4(None, ctypes.byref(cache()), ctypes.byref(a)), EINVAL, text)
 
 
-def test_most_tokens_of_a_cache_call(lib):  # noqa: F811
-    """A launch has fewer than 2^32 threads along an axis: 2^24 - 1 workgroups."""
-    st = (ctypes.c_int64 * 2)(0, 0)
-    for fn in (lib.qph_cache4_write, lib.qph_cache4_read):
-        for heads, dh, most in ((64, 256, 4 * ((1 << 24) - 1)), (1, 32, 4 * 64 * ((1 << 24) - 1))):
-            c = cache(heads=heads, dh=dh)
-            for tokens, code, text in ((most, EINVAL, "null context"), (most + 1, EUNSUPPORTED, "too many tokens")):
-                refused(lib, fn(None, ctypes.byref(c), A, A, 0, tokens, st, st, A), code, text)
-
-
 def test_most_blocks_of_a_weight(lib):  # noqa: F811
+    """A launch has fewer than 2^32 threads along an axis: 2^24 - 1 workgroups."""
     for k, groups in ((128, 4), (1 << 20, 1 << 15)):
         rows = ((1 << 24) - 1) * 256 // groups
         for n, code, text in ((rows, EINVAL, "null context"), (rows + 1, EUNSUPPORTED, "blocks")):

@@ -19,7 +19,7 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("heads,dh,page,tokens", [
     (8, 128, 64, 8192 + 3), (3, 64, 32, 81920 + 27), (1, 32, 16, 524288 + 4 * 64 + 1)])
 def test_cache_many_tokens(gpu, dtype, heads, dh, page, tokens):
-    """Writes and reads with four tokens in flight a thread (from 8192 workgroups'
+    """Long writes, and reads with four tokens in flight a thread (from 8192 workgroups'
     tokens on), the last group ragged, padded and bad slots among them: the bits of
     the same tokens in short calls; some of them against the definition."""
     from qppocr_amd import ops
@@ -240,3 +240,24 @@ def test_linear_activations(gpu, dtype, name, rows):
         want = v * np.clip(v + a, 0, b) / c
         tol = (b + np.abs(v)) / c * tol + 4 * u * np.abs(v) * (np.abs(v) + a + b) / c
     close(host(y), want, tol + half_step(gpu, t, want) * 1.001, name)
+
+
+def test_cache_write_of_more_tokens_than_a_launch(gpu):
+    """More workgroups than one launch takes (2^24 - 1, a token each): one row of keys
+    and values for all tokens, all but a few at both sides of the border skipped."""
+    from qppocr_amd import ops
+    heads, dh, page, border = 64, 256, 16, (1 << 24) - 1
+    print("cache4 write, two launches", flush=True)
+    rng = np.random.default_rng(7)
+    c = make_cache(gpu, rng, 2, page, heads, dh)
+    want = [x.reshape(2 * page, heads, dh).copy() for x in numbers(c)]
+    kv = gpu.from_numpy(rng.standard_normal((2, heads, dh)).astype(np.float32)).cuda().half()
+    n = border + 5
+    slots = gpu.full((n,), -1, dtype=gpu.int64, device="cuda")
+    for t, slot in ((0, 3), (border - 1, 30), (border, 9), (n - 1, 17)):
+        slots[t] = slot
+    ops.cache4_write(c, kv[0].expand(n, heads, dh), kv[1].expand(n, heads, dh), slots)
+    for i, x in enumerate(numbers(c)):
+        code, scale = encode(host(kv[i]))
+        want[i][[3, 30, 9, 17]] = decode((code[..., 0::2] | code[..., 1::2] << 4).astype(np.uint8), scale)
+        close(x.reshape(2 * page, heads, dh), want[i], 0.0, f"stored {'kv'[i]}")
