@@ -345,8 +345,9 @@ QPH_API int qph_quantize4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t ro
  * residual[rows, n], W [n][kp] as qph_quantize4 leaves it.  x, bias, residual
  * and y are of dtype; x has rows x_stride elements apart, y and residual are
  * contiguous (residual may be y); bias, act and residual may be NULL.  The
- * products are exact, sums are float32, y is rounded once.  GELU uses the
- * error function itself, not the approximation of qph_linear. */
+ * products are exact (bits of a float32 x below 2^-126 count as zeros), sums
+ * are float32, y is rounded once.  GELU uses the error function itself, not the
+ * approximation of qph_linear. */
 QPH_API int qph_linear4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t x_stride,
                         const void* codes, const void* scales, const void* bias, int64_t rows,
                         int64_t k, int64_t n, const qph_act* act, const void* residual, void* y);
@@ -389,16 +390,17 @@ QPH_API int qph_cache4_read(qph_ctx* ctx, const qph_cache4* cache, void* k, void
  *   lse = log sum_j exp(scale q . k_j)     (float32 [tokens][heads], or NULL)
  * A row that sees no key gets zeros and -infinity.  Rows that no sequence has
  * are left as they were.  out may be q itself (with its strides); its elements
- * share no memory with q's otherwise, nor with each other.  max_new and max_len (host) bound the sequences' new
- * and cached tokens; they choose the work's split, and longer ones only run
- * slower.  lens are cut at max_pages pages.  Scores, sums and the running
- * maximum are float32 (scores of any finite size; one past float32's range
- * makes its row NaN), keys and values exact, the probabilities kept to 16
- * bits (24 for float32) in the second product.
+ * share no memory with q's otherwise, nor with each other.  max_new and max_len
+ * (host) bound the sequences' new and cached tokens; they choose the work's
+ * split, and longer ones only run slower.  lens are cut at max_pages pages and
+ * at 2^31 - 256 keys.  Scores, sums and the running maximum are float32 (scores
+ * of any size; one past float32's range counts as an infinity, and +infinity
+ * makes its row NaN), keys and values exact, the probabilities kept to 16 bits
+ * (24 for float32) in the second product.
  * page_table, lens and starts are device memory.  The workspace (device, of
  * qph_attention_cache4_workspace bytes for the same arguments, which depend on
- * no device data; 16-byte aligned) is this call's until it has run; calls that may overlap need
- * one each. */
+ * no device data; 16-byte aligned) is this call's until it has run; calls that
+ * may overlap need one each. */
 typedef struct {
   const void* q;              /* [tokens][heads][dh], strides {token, head} */
   void* out;                  /* the same shape */

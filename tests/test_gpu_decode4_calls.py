@@ -296,3 +296,46 @@ def test_attention_in_place(gpu, dtype, form):
     assert ops.attention_cache4(q, *args, out=q, **kw) is q
     assert (host(q) == host(want)).all()
     assert (packed[:, :2] == kept[:, :2]).all() and (packed[:, 2 + heads * group:] == kept[:, 2 + heads * group:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_attention_scores_past_the_largest_number(gpu, dtype, form):
+    """Scores that overflow float32: minus infinity weighs nothing, plus infinity makes
+    its row NaN; rows beside them do not change by a bit."""
+    from qppocr_amd import ops
+    print("attention overflowing scores", dtype, form, flush=True)
+    rng = np.random.default_rng(19)
+    heads, group, page, news, lens, _ = FORMS[form]
+    dh, t = 64, getattr(gpu, dtype)
+
+    def keys(rng, shape):
+        code = np.zeros(shape, dtype=np.int64)
+        code[..., 0] = rng.choice([0, 0, 15], shape[:-1])            # 0 or -6
+        code[..., 32:] = rng.choice([0, 2, 4, 10, 12], shape[:-1] + (32,))
+        return code, np.full(shape[:-1] + (2,), 127)
+    c, table = form_cache(gpu, rng, form, dh, keys)
+    q = np.zeros((sum(news), heads * group, dh))
+    q[..., 32:] = rng.integers(-1, 2, q[..., 32:].shape)
+    plain = gpu.from_numpy(q.astype(np.float32)).cuda().to(t)
+    q[0::3, :, 0], q[1::3, :, 0] = 3e38, -3e38
+    q = gpu.from_numpy(q.astype(np.float32)).cuda().to(t)
+    st, i32 = [0] + list(np.cumsum(news)), dict(dtype=gpu.int32, device="cuda")
+    ordinary = host(ops.attention_cache4(plain, c, gpu.tensor(table, **i32), gpu.tensor(lens, **i32), 1.0,
+                                         starts=gpu.tensor(st, **i32), max_new=max(news), max_len=max(lens)))
+    kept = 2.0 ** -23 if dtype == "float32" else 2.0 ** -16
+    for name, y, lse, qd, k, v, (b, i) in run_form(gpu, c, form, table, q, 1.0):
+        h = int(name.split()[-1])
+        hidden = k[:, 0] < 0
+        if qd[0] < 0 and hidden.any():
+            assert np.isnan(y).all() and np.isnan(lse), name
+        elif qd[0] > 0 and hidden.all():
+            assert (y == 0).all() and lse == -np.inf, name
+        elif qd[0] > 0:
+            z = np.where(hidden, -np.inf, k[:, 32:] @ qd[32:])
+            p = np.exp(z - z.max())
+            off = np.where(hidden, 0.0, 2.0 ** -22 * (1 + np.abs(np.where(hidden, 0.0, z - z.max()))))
+            want, d, tol = mean_of_values(p, off, v, kept)
+            close(y, want, tol + half_step(gpu, t, want) * 1.001, name)
+        else:
+            assert (y == ordinary[st[b] + i, h]).all(), name
