@@ -341,7 +341,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
         }
       }
       // masks, only where a border lies in the tile or a page is none
-      if (careful || j0 < all_lo || j0 + 32 > all_hi || !(pg.there[0] && pg.there[1])) {
+      if (j0 < all_lo || j0 + 32 > all_hi || !(pg.there[0] && pg.there[1])) {
 #pragma unroll
         for (int q = 0; q < NQ; q++)
 #pragma unroll
@@ -540,6 +540,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
       }
       careful = __any(careful);
       if (!careful) break;
+      all_lo = INT32_MAX;        // the masks' part of every tile takes the maximum off
 #pragma unroll
       for (int q = 0; q < NQ; q++) {
         const float sum = column_sum(l[q]);
@@ -601,6 +602,10 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
       }
     }
     constexpr int NR = WS == 4 ? 1 : 4;
+    // (out of the compiler's sight, which otherwise holds the stores' addresses through
+    // the walk: one long cache in float16 41.4 us, 40.6 so)
+    int kgs = kg;
+    if constexpr (WS == 4) asm volatile("" : "+v"(kgs));
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
       if (!live[q]) continue;
@@ -614,7 +619,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
         if (l[q] == 0.0f) continue;
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-          float* p = a.part_o + part * DH + 2 * W * (4 * kg + (WS == 4 ? wave : r));
+          float* p = a.part_o + part * DH + 2 * W * (4 * kgs + (WS == 4 ? wave : r));
 #pragma unroll
           for (int x = 0; x < 2 * W; x++) p[x] = o[q][x][r];
         }
@@ -625,7 +630,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
 #pragma unroll
         for (int r = 0; r < NR; r++) {
           typename E::type* p = (typename E::type*)a.out + tok[q] * a.ot + head[q] * a.oh +
-                                2 * W * (4 * kg + (WS == 4 ? wave : r));
+                                2 * W * (4 * kgs + (WS == 4 ? wave : r));
           typename E::type t[2 * W];
 #pragma unroll
           for (int x = 0; x < 2 * W; x++) t[x] = (typename E::type)(o[q][x][r] * inv);
