@@ -537,56 +537,68 @@ __global__ __launch_bounds__(512) void linear4_rows_kernel(const typename E::typ
   }
 }
 
+// HIP takes less than 2^32 threads along an axis of a launch.
+static int linear4_fits(dim3 grid, int threads) {
+  if ((uint64_t)grid.x * threads >> 32)
+    return fail(QPH_EUNSUPPORTED, "linear4: too many columns for one call");
+  return QPH_OK;
+}
+
+// (The launchers take the stream's context; without one they only check the launch.)
 template <typename E, int NQ, int NT, int U>
-static int launch_linear4_few(const Lin4& a, hipStream_t s) {
+static int launch_linear4_few(const Lin4& a, const qph_ctx* ctx) {
   // up to 8 waves along k, with a group of chunks each
   const int part = std::max(NQ * 16 * NT * 16 * 4, NQ * 2 * (int)sizeof(typename E::type) * 1024);
   int waves = 8;
   while (waves > 1 && (waves / 2) * U >= a.chunks) waves /= 2;
-  if (waves * part > 65536) QPH_TRY(allow_full_lds((const void*)linear4_few_kernel<E, NQ, NT, U>));
   const dim3 grid(ceil_div(a.n, 16 * NT), ceil_div(a.rows, 16 * NQ));
-  hipLaunchKernelGGL((linear4_few_kernel<E, NQ, NT, U>), grid, dim3(64 * waves), waves * part, s,
+  QPH_TRY(linear4_fits(grid, 64 * waves));
+  if (!ctx) return QPH_OK;
+  if (waves * part > 65536) QPH_TRY(allow_full_lds((const void*)linear4_few_kernel<E, NQ, NT, U>));
+  hipLaunchKernelGGL((linear4_few_kernel<E, NQ, NT, U>), grid, dim3(64 * waves), waves * part, ctx->stream,
                      (const typename E::type*)a.x, a.codes, a.scales, a.xs, (int)a.rows, (int)a.k,
                      (int)a.n, (int)a.chunks, a);
   return launch_check("linear4_few_kernel");
 }
 
 template <typename E, int NQ, int NT, int D>
-static int launch_linear4_rows(const Lin4& a, hipStream_t s) {
+static int launch_linear4_rows(const Lin4& a, const qph_ctx* ctx) {
   constexpr int TS = E::terms == 3 ? 3 : 1;
   const int lds = std::max(4 * 4 * NQ * TS * 1024, 2 * 16 * NQ * 64 * NT * 4);
-  if (lds > 65536) QPH_TRY(allow_full_lds((const void*)linear4_rows_kernel<E, NQ, NT, D>));
   const dim3 grid(ceil_div(a.n, 64 * NT), ceil_div(a.rows, 16 * NQ));
-  hipLaunchKernelGGL((linear4_rows_kernel<E, NQ, NT, D>), grid, dim3(512), lds, s,
+  QPH_TRY(linear4_fits(grid, 512));
+  if (!ctx) return QPH_OK;
+  if (lds > 65536) QPH_TRY(allow_full_lds((const void*)linear4_rows_kernel<E, NQ, NT, D>));
+  hipLaunchKernelGGL((linear4_rows_kernel<E, NQ, NT, D>), grid, dim3(512), lds, ctx->stream,
                      (const typename E::type*)a.x, a.codes, a.scales, a.xs, (int)a.rows, (int)a.k,
                      (int)a.n, (int)a.chunks, a);
   return launch_check("linear4_rows_kernel");
 }
 
 template <typename E, int NQ, int U>
-static int launch_linear4_few_nt(const Lin4& a, hipStream_t s) {
+static int launch_linear4_few_nt(const Lin4& a, const qph_ctx* ctx) {
   // Columns a workgroup: so many that one round of workgroups, one to each of
   // the 256 CUs, takes them, at most 64 (48 for two row tiles, whose registers
   // end there).  8 rows of 4096 x 12288 (768 column tiles) by one, two, three
   // and four tiles: 11.2, 11.4, 9.2 and 11.0 us; 16 of 4096 x 4096 (256): 5.9,
   // 7.5, 8.9 and 10.6.
   const int64_t tiles = (a.n + 15) / 16 * ((a.rows + 16 * NQ - 1) / (16 * NQ));
-  if (tiles <= 256) return launch_linear4_few<E, NQ, 1, U>(a, s);
-  if (tiles <= 512) return launch_linear4_few<E, NQ, 2, U>(a, s);
+  if (tiles <= 256) return launch_linear4_few<E, NQ, 1, U>(a, ctx);
+  if (tiles <= 512) return launch_linear4_few<E, NQ, 2, U>(a, ctx);
   if constexpr (NQ == 1) {
     // past 1024 tiles as many rounds as four tiles make, but even ones: 1 x 4096
     // x 20000 by three 15.1 us, by four 17.5, 16 x 256 x 18709 5.1 and 5.8
     const int64_t round = (tiles + 1023) / 1024 * 256;
-    if (tiles > 3 * round) return launch_linear4_few<E, NQ, 4, U>(a, s);
+    if (tiles > 3 * round) return launch_linear4_few<E, NQ, 4, U>(a, ctx);
   }
-  return launch_linear4_few<E, NQ, 3, U>(a, s);
+  return launch_linear4_few<E, NQ, 3, U>(a, ctx);
 }
 
 template <typename E>
-static int launch_linear4(const Lin4& a, hipStream_t s) {
+static int launch_linear4(const Lin4& a, const qph_ctx* ctx) {
   constexpr bool f32 = E::terms == 3;
   // up to 16 rows: 16 x 4096 x 32768 22 us (float32 33), 33 (52) by more rows' kernel
-  if (a.rows <= 16) return launch_linear4_few_nt<E, 1, 2>(a, s);
+  if (a.rows <= 16) return launch_linear4_few_nt<E, 1, 2>(a, ctx);
   // More rows cost their turning and, in float32, their split into terms in
   // every workgroup here; the other kernel shares them between more columns,
   // with less of the weights in flight.  So here while one round of workgroups
@@ -599,19 +611,19 @@ static int launch_linear4(const Lin4& a, hipStream_t s) {
   // its smallest workgroups: 20 x 1024 x 18709 7.6 and 11.6 us, 32 x 4096 x 32768
   // 32.0 and 33.9, but 32 x 4096 x 16384 21.9 and 17.0)
   if (a.rows <= (f32 ? 32 : 64) && (round || (!f32 && a.rows <= 32 && !round_32x64)))
-    return launch_linear4_few_nt<E, 2, f32 ? 1 : 2>(a, s);
+    return launch_linear4_few_nt<E, 2, f32 ? 1 : 2>(a, ctx);
   // Then the smallest workgroups that one round takes: 32 rows x 64 columns (128
   // x 4096 x 4096 16 us, 22 with 64 rows; in float32 35, 48 with 48 rows x 128
   // columns), 64 x 64 (256 x 4096 x 4096 23.4; 26.5 with 32 rows, 31.5 with 128
   // columns).  Past that the ones that do most with what they load: 64 x 128
   // (2048 x 4096 x 12288 343 us, 470 with 64 columns), in float32 48 x 128 (779
   // us, 1425 with 32 x 64).
-  if (round_32x64) return launch_linear4_rows<E, 2, 1, 4>(a, s);
+  if (round_32x64) return launch_linear4_rows<E, 2, 1, 4>(a, ctx);
   if constexpr (f32) {
-    return launch_linear4_rows<E, 3, 2, 2>(a, s);
+    return launch_linear4_rows<E, 3, 2, 2>(a, ctx);
   } else {
-    if ((a.n + 63) / 64 * ((a.rows + 63) / 64) <= 256) return launch_linear4_rows<E, 4, 1, 4>(a, s);
-    return launch_linear4_rows<E, 4, 2, 2>(a, s);
+    if ((a.n + 63) / 64 * ((a.rows + 63) / 64) <= 256) return launch_linear4_rows<E, 4, 1, 4>(a, ctx);
+    return launch_linear4_rows<E, 4, 2, 2>(a, ctx);
   }
 }
 
@@ -738,12 +750,9 @@ QPH_API int qph_linear4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t x_st
   if (rows && (!x || !codes || !scales || !y)) return fail(QPH_EINVAL, "linear4: NULL argument");
   if ((uintptr_t)codes % 16 || (uintptr_t)scales % 4)
     return fail(QPH_EINVAL, "linear4: codes are not 16-byte or scales not 4-byte aligned");
-  // columns, rows and k are counted in 32 bits, row tiles by the grid's second axis;
-  // 512 threads take 48 columns or more where there are many
-  if (n > (1 << 28) || k > (1 << 30) || rows > 65535 * 16)
-    return fail(QPH_EUNSUPPORTED, "linear4: more than 2^28 columns, 2^30 inputs or 1048560 rows");
-  if (!ctx) return fail(QPH_EINVAL, "null context");
-  if (rows == 0) return QPH_OK;
+  // columns, rows and k are counted in 32 bits, row tiles by the grid's second axis
+  if (n > (1 << 30) || k > (1 << 30) || rows > 65535 * 16)
+    return fail(QPH_EUNSUPPORTED, "linear4: more than 2^30 columns or inputs, or 1048560 rows");
   Lin4 a{};
   a.x = x; a.xs = x_stride;
   a.codes = (const unsigned char*)codes;
@@ -752,11 +761,20 @@ QPH_API int qph_linear4(qph_ctx* ctx, const void* x, int32_t dtype, int64_t x_st
   a.rows = rows; a.k = k; a.n = n;
   a.chunks = (k + 127) / 128;
   a.act = make_act(act);
+  auto launch = [&](const qph_ctx* on) {
+    if (rows == 0) return (int)QPH_OK;
+    if (dtype == QPH_F32) return launch_linear4<F32>(a, on);
+    if (dtype == QPH_F16) return launch_linear4<F16>(a, on);
+    return launch_linear4<BF16>(a, on);
+  };
+  if (!ctx) {
+    QPH_TRY(launch(nullptr));
+    return fail(QPH_EINVAL, "null context");
+  }
+  if (rows == 0) return QPH_OK;
   OnDevice dev(ctx);
   QPH_TRY(dev.rc());
-  if (dtype == QPH_F32) return launch_linear4<F32>(a, ctx->stream);
-  if (dtype == QPH_F16) return launch_linear4<F16>(a, ctx->stream);
-  return launch_linear4<BF16>(a, ctx->stream);
+  return launch(ctx);
 }
 
 QPH_API int qph_cache4_write(qph_ctx* ctx, const qph_cache4* cache, const void* k, const void* v,

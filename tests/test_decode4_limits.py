@@ -25,10 +25,21 @@ def test_most_blocks_of_a_weight(lib):  # noqa: F811
             refused(lib, lib.qph_quantize4(None, A, 1, n, k, 0, 1, A, A), code, text)
 
 
-def test_most_columns_of_a_linear(lib):  # noqa: F811
-    for rows in (1, 40, 3000):
-        for n, code, text in ((1 << 28, EINVAL, "null context"), ((1 << 28) + 1, EUNSUPPORTED, "2^28 columns")):
-            refused(lib, lib.qph_linear4(None, A, 0, 64, A, A, None, rows, 64, n, None, None, A), code, text)
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows,k,columns,threads", [
+    (1, 2048, 64, 512), (16, 4096, 64, 512), (1, 1024, 64, 256), (3, 512, 64, 128), (1, 256, 64, 64), (17, 2048, None, 512),
+    (3000, 4096, 128, 512), (200, 64, 128, 512)])
+def test_most_columns_of_a_linear(lib, dtype, rows, k, columns, threads):  # noqa: F811
+    """Every column count whose workgroups (of 64 columns, with more rows 128) stay below
+    2^32 threads, and 2^30 at most."""
+    def call(n):
+        return lib.qph_linear4(None, A, dtype, k, A, A, None, rows, k, n, None, None, A)
+    if columns is None:                            # (48 or 128 by the type)
+        columns = 128 if dtype == 0 else 48
+    most = min(columns * (((1 << 32) - 1) // threads), 1 << 30)
+    refused(lib, call(most), EINVAL, "null context")
+    refused(lib, call(most + 1), EUNSUPPORTED, "columns")
+    refused(lib, call(1 << 26), EINVAL, "null context")
 
 
 def test_most_sequences_of_an_attention(lib):  # noqa: F811
