@@ -716,8 +716,9 @@ def cache4_write(cache, k, v, slots):
 
 def cache4_read(cache, slots, dtype=torch.float32, out=None):
     """The tokens of slots, int64 [tokens], as (k, v) [tokens, heads, dh] of
-    dtype; zeros for a slot outside the pool.  out: such a pair to write into
-    (tokens and heads of any strides)."""
+    dtype; zeros for a slot outside the pool.  out: such a pair to write into, whose
+    type counts instead (tokens and heads of any strides, no two elements in one
+    place)."""
     if slots.dim() != 1:
         raise ValueError("cache4_read: slots [tokens]")
     n = slots.shape[0]
@@ -765,9 +766,9 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
     pages and cached tokens, its new ones the last of them.  starts int32
     [batch + 1]: sequence b's new tokens are q[starts[b]:starts[b + 1]], at most
     max_new (needed then); without starts every sequence has tokens / batch.
-    max_len bounds lens (default: all of the table's pages).  out may be q itself, and
-    shares no memory with it otherwise.  causal hides
-    later keys, window > 0 all but the last `window` up to a token's own.  A
+    max_len bounds lens (default: all of the table's pages).  causal hides later
+    keys, window > 0 all but the last `window` up to a token's own.  out may be q
+    itself, and shares no memory with it otherwise, nor its elements any.  A
     row that sees no key is zero; rows of no sequence keep what out holds.
     Returns out, or (out, lse) with the sums' logarithms, float32 [tokens,
     heads] (-infinity where no key is seen; a new tensor's rows of no sequence

@@ -1,6 +1,6 @@
-"""The 4-bit operators' calls that a program makes in less usual ways, and the
-forms of their kernels that only particular sizes reach, against the same
-definitions in 64 bits as the other tests of these operators."""
+"""The 4-bit operators' calls that a program makes in less usual ways (other default
+types, scores and values of any size, bounds far from the work, in place), against
+the same definitions in 64 bits as the other tests of these operators."""
 import math
 
 import numpy as np
