@@ -421,6 +421,105 @@ QPH_API int qph_attention_cache4_workspace(const qph_cache4* cache, const qph_at
                                            size_t* bytes);
 QPH_API int qph_attention_cache4(qph_ctx* ctx, const qph_cache4* cache, const qph_attn4* args);
 
+/* Attention where a row sees more than a run of keys.  sinks: with a window, the
+ * first `sinks` keys of the sequence stay visible (j <= p and (j > p - window or
+ * j < sinks)); without one they are visible anyway.  tree: the new tokens of a
+ * sequence are drafted as a tree.  Row t of the masks, tree[t * tree_words ..], has
+ * bit i (of word i / 64) for each new token i of the sequence that token t sees,
+ * itself among them; of the context, the keys j < c = lens[b] - n before the n new
+ * tokens, it sees all, or with a window those with j > p - window or j < sinks,
+ * where p = c - 1 + its row's bits (a path's end stands as many places behind the
+ * context as the path is long).  A window hides no drafted token, causal is not
+ * used, and bits from n on count for nothing.  tree_words is 0 without a tree and
+ * max_new / 64 rounded up at least with one (drafted tokens past the words are not
+ * seen).  Everything else is as in qph_attention_cache4, the workspace's rules too. */
+typedef struct {
+  int64_t sinks;
+  const uint64_t* tree;       /* [tokens][tree_words], device */
+  int64_t tree_words;
+} qph_attn4_mask;
+QPH_API int qph_attention_mask4_workspace(const qph_cache4* cache, const qph_attn4* args,
+                                          const qph_attn4_mask* mask, size_t* bytes);
+QPH_API int qph_attention_mask4(qph_ctx* ctx, const qph_cache4* cache, const qph_attn4* args,
+                                const qph_attn4_mask* mask);
+
+/* A step's pages, slots, positions and masks from its lengths, all on the device.
+ * Sequence b has lens[b] cached tokens (0 to what its row of the table holds, at
+ * most 2^31 - 256) on the first lens[b] / page_size rounded up pages of its row,
+ * and grows by news[b] tokens, or shrinks by -news[b] (to 0 at least).  Free pages
+ * are ring[i % ring_n] for ends[0] <= i < ends[1]; a ring with room for every page
+ * of the pool never runs over (pages given back to a full one are dropped).
+ *   starts    sums of the positive news, cut at tokens (the rows of the outputs)
+ *   lens      after the step
+ *   slots     for a row: page * page_size + place, or -1
+ *   positions for a row: lens[b] + its index, with parents + its depth in the tree
+ *   tree      with parents: the masks of qph_attention_mask4 (tree_words a row)
+ *   ends      after the step: pages are taken from ends[0] on and given back at
+ *             ends[1]; pages given back can be taken by the next call
+ * Sequences take pages in their order.  One whose pages are not all there, that
+ * its row of the table does not hold or whose rows end past `tokens` is not
+ * granted: its length stays, its rows' slots are -1 and it takes no page (nor does
+ * any later one that needs some, where pages ran out).  page_table is written where
+ * pages are taken (entries behind a sequence's last page mean nothing), the ring
+ * where they are given back.  parents[t] is the index of row t's parent among its
+ * sequence's new tokens, smaller than its own; anything else makes it a child of
+ * the context.  Rows of no sequence get slot -1, position 0 and no bits.  The
+ * outputs share no memory with the inputs.  page_size is a power of two, 16 to
+ * 32768.  workspace: qph_cache4_extend_workspace bytes, as for the attention. */
+typedef struct {
+  int32_t* page_table;        /* [batch][max_pages], rows table_stride apart */
+  int64_t table_stride, max_pages, batch;
+  const int32_t *lens, *news; /* [batch] */
+  int32_t* ring;              /* [ring_n] */
+  int64_t ring_n;
+  const int64_t* ends;        /* [2] */
+  int64_t tokens;
+  const int32_t* parents;     /* [tokens], or NULL */
+  int64_t tree_words;
+  int32_t *out_starts, *out_lens;   /* [batch + 1], [batch] */
+  int64_t* out_slots;         /* [tokens] */
+  int32_t* out_positions;     /* [tokens] */
+  int64_t* out_ends;          /* [2] */
+  uint64_t* out_tree;         /* [tokens][tree_words], with parents */
+  int32_t page_size;
+  void* workspace;
+  size_t workspace_bytes;
+} qph_extend4;
+QPH_API int qph_cache4_extend_workspace(int64_t batch, size_t* bytes);
+QPH_API int qph_cache4_extend(qph_ctx* ctx, const qph_extend4* args);
+
+/* Tokens' keys and values from slots to slots, as they are held; all are read
+ * before any is written, so that a slot may be left and taken in one call (an
+ * accepted path behind its context).  A pair with a slot outside the pool is
+ * skipped; the dst of one call must differ from each other.  workspace (16-byte
+ * aligned): qph_cache4_move_workspace bytes, as for the attention. */
+QPH_API int qph_cache4_move_workspace(const qph_cache4* cache, int64_t tokens, size_t* bytes);
+QPH_API int qph_cache4_move(qph_ctx* ctx, const qph_cache4* cache, const int64_t* src,
+                            const int64_t* dst, int64_t tokens, void* workspace,
+                            size_t workspace_bytes);
+
+/* Rotation by positions: pair i < pairs of a head, its elements i and pairs + i, or
+ * 2 i and 2 i + 1 (neighbours), turns by the angle t = positions[axes[i]][token] *
+ * turns[i] / 2^64 turns:
+ *   (u, v) -> (u cos t - v sin t, u sin t + v cos t)
+ * or with inverse by -t (the transpose, which is the gradient's rotation too).  The
+ * product is exact modulo a turn.  Elements from 2 pairs on are copied.  x and out
+ * [tokens][heads][dh] have strides {token, head}; out may be x itself (with its
+ * strides) and shares no memory with it otherwise.  Cosines, sines and products are
+ * float32, out is rounded once. */
+typedef struct {
+  const void* x;
+  void* out;
+  int64_t x_strides[2], out_strides[2];
+  int64_t tokens;
+  const void* positions;      /* int32, or int64 with positions_64 */
+  int64_t position_strides[2];      /* {axis, token}; 0 for one position on all axes */
+  const uint64_t* turns;      /* [pairs] 2^-64 turns a position (device) */
+  const int32_t* axes;        /* [pairs], each below n_axes (device) */
+  int32_t dtype, heads, dh, pairs, n_axes, positions_64, neighbours, inverse;
+} qph_rotary_args;
+QPH_API int qph_rotary(qph_ctx* ctx, const qph_rotary_args* args);
+
 /* ------------------------------------------------------------- session */
 
 /* A static det or rec graph (the optimised graph the DeviceContext receives,

@@ -96,6 +96,31 @@ class Attn4(ctypes.Structure):
                 ("window", I32), ("workspace", P), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class Attn4Mask(ctypes.Structure):
+    """qph_attn4_mask: first tokens that stay visible, masks of drafted trees."""
+    _fields_ = [("sinks", I64), ("tree", P), ("tree_words", I64)]
+
+
+class Extend4(ctypes.Structure):
+    """qph_extend4: a step's lengths and what is made of them."""
+    _fields_ = [("page_table", P), ("table_stride", I64), ("max_pages", I64), ("batch", I64),
+                ("lens", P), ("news", P), ("ring", P), ("ring_n", I64), ("ends", P),
+                ("tokens", I64), ("parents", P), ("tree_words", I64), ("out_starts", P),
+                ("out_lens", P), ("out_slots", P), ("out_positions", P), ("out_ends", P),
+                ("out_tree", P), ("page_size", I32), ("workspace", P),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """qph_rotary_args: a rotation by positions."""
+    _fields_ = [("x", P), ("out", P), ("x_token", I64), ("x_head", I64),                   # x_strides
+                ("out_token", I64), ("out_head", I64),                                 # out_strides
+                ("tokens", I64), ("positions", P), ("p_axis", I64), ("p_token", I64),  # position_strides
+                ("turns", P), ("axes", P), ("dtype", I32), ("heads", I32), ("dh", I32),
+                ("pairs", I32), ("n_axes", I32), ("positions_64", I32), ("neighbours", I32),
+                ("inverse", I32)]
+
+
 # exported symbol -> (argtypes, restype); every symbol include/qppocr_hip.h declares
 SIGNATURES = {
     "qph_ctx_create": ([ctypes.c_int, ctypes.POINTER(P)], ctypes.c_int),
@@ -152,6 +177,17 @@ SIGNATURES = {
     "qph_attention_cache4_workspace": ([ctypes.POINTER(Cache4), ctypes.POINTER(Attn4),
                                         ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "qph_attention_cache4": ([P, ctypes.POINTER(Cache4), ctypes.POINTER(Attn4)], ctypes.c_int),
+    "qph_attention_mask4_workspace": ([ctypes.POINTER(Cache4), ctypes.POINTER(Attn4),
+                                       ctypes.POINTER(Attn4Mask), ctypes.POINTER(ctypes.c_size_t)],
+                                      ctypes.c_int),
+    "qph_attention_mask4": ([P, ctypes.POINTER(Cache4), ctypes.POINTER(Attn4),
+                             ctypes.POINTER(Attn4Mask)], ctypes.c_int),
+    "qph_cache4_extend_workspace": ([I64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "qph_cache4_extend": ([P, ctypes.POINTER(Extend4)], ctypes.c_int),
+    "qph_cache4_move_workspace": ([ctypes.POINTER(Cache4), I64, ctypes.POINTER(ctypes.c_size_t)],
+                                  ctypes.c_int),
+    "qph_cache4_move": ([P, ctypes.POINTER(Cache4), P, P, I64, P, ctypes.c_size_t], ctypes.c_int),
+    "qph_rotary": ([P, ctypes.POINTER(RotaryArgs)], ctypes.c_int),
     "qph_net_create": ([P, ctypes.POINTER(NetSpec), ctypes.POINTER(P), ctypes.POINTER(P)],
                        ctypes.c_int),
     "qph_net_destroy": ([P], ctypes.c_int),

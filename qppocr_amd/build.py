@@ -19,7 +19,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["qph_runtime.hip", "qph_gemm.hip", "qph_conv.hip", "qph_block.hip", "qph_rows.hip",
            "qph_net.hip", "qph_aux.hip", "qph_plan.hip", "qph_head.hip", "qph_fp4.hip",
-           "qph_attn4.hip"]
+           "qph_attn4.hip", "qph_mask4.hip", "qph_mask4_f16.hip", "qph_mask4_f32.hip",
+           "qph_step4.hip"]
 
 CFLAGS = [
     "--offload-arch=gfx950",
@@ -40,7 +41,7 @@ CFLAGS = [
 # latency from end to end, so the first arguments come in registers with the
 # wave rather than by a load it has to wait for.
 EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm",
-             "-amdgpu-kernarg-preload-count=16"] for f in ("qph_fp4.hip", "qph_attn4.hip")}
+             "-amdgpu-kernarg-preload-count=16"] for f in SOURCES[SOURCES.index("qph_fp4.hip"):]}
 
 # host-code sanitizers only (the device code is built as usual): each
 # -fsanitize= goes to the host compilation alone

@@ -15,8 +15,11 @@ torch's current stream of the tensors' device, in its order, and may be captured
 into a graph; they compute no gradients and refuse tensors that require one.
 Errors raise QphError (no silent fallback).
 """
+import collections
 import ctypes
+import fractions
 import functools
+import math
 import threading
 
 import torch
@@ -745,20 +748,26 @@ def cache4_read(cache, slots, dtype=torch.float32, out=None):
 
 @functools.lru_cache(maxsize=1024)
 def _workspace4(pages, page, heads, dh, *sizes):
-    """qph_attention_cache4_workspace, which sees the sizes alone."""
+    """qph_attention_cache4_workspace, which sees the sizes alone (with sinks and a
+    tree's words behind them qph_attention_mask4_workspace)."""
     c = _lib.Cache4(256, 256, 256, 256, pages, page, heads, dh)
     a = _lib.Attn4()
     (a.dtype, a.heads, a.tokens, a.batch, a.max_pages, a.max_new, a.max_len, a.causal, a.window,
-     a.starts) = sizes
+     a.starts) = sizes[:10]
     a.scale = 1.0
     size = ctypes.c_size_t()
-    check(_lib.load().qph_attention_cache4_workspace(ctypes.byref(c), ctypes.byref(a),
-                                                     ctypes.byref(size)))
+    if len(sizes) == 10:
+        check(_lib.load().qph_attention_cache4_workspace(ctypes.byref(c), ctypes.byref(a),
+                                                         ctypes.byref(size)))
+    else:
+        mask = _lib.Attn4Mask(sizes[10], 256, sizes[11])
+        check(_lib.load().qph_attention_mask4_workspace(ctypes.byref(c), ctypes.byref(a),
+                                                        ctypes.byref(mask), ctypes.byref(size)))
     return size.value
 
 
 def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=None, max_len=None,
-                     causal=True, window=0, lse=False, out=None):
+                     causal=True, window=0, lse=False, out=None, sinks=0):
     """Attention of new tokens q [tokens, heads, dh] over a Cache4 that holds
     their keys and values already.
 
@@ -767,13 +776,36 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
     [batch + 1]: sequence b's new tokens are q[starts[b]:starts[b + 1]], at most
     max_new (needed then); without starts every sequence has tokens / batch.
     max_len bounds lens (default: all of the table's pages).  causal hides later
-    keys, window > 0 all but the last `window` up to a token's own.  out may be q
-    itself, and shares no memory with it otherwise, nor its elements any.  A
-    row that sees no key is zero; rows of no sequence keep what out holds.
+    keys, window > 0 all but the last `window` up to a token's own and the
+    sequence's first `sinks`.  out may be q itself, and shares no memory with it
+    otherwise, nor its elements any.  A row that sees no key is zero; rows of no
+    sequence keep what out holds.
     Returns out, or (out, lse) with the sums' logarithms, float32 [tokens,
     heads] (-infinity where no key is seen; a new tensor's rows of no sequence
     are undefined)."""
-    what = "attention_cache4"
+    return _attention4("attention_cache4", q, cache, page_table, lens, scale, starts, max_new, max_len,
+                       causal, window, sinks, None, lse, out)
+
+
+def attention_tree4(q, cache, page_table, lens, scale, tree, starts=None, max_new=None, max_len=None,
+                    window=0, sinks=0, lse=False, out=None):
+    """attention_cache4 of new tokens that were drafted as trees: tree int64
+    [tokens, words], contiguous, has in row t bit i % 64 of word i // 64 for each
+    new token i of its sequence that token t sees, itself among them (cache4_extend
+    makes such masks from parents).  Of the context (the cached tokens before the
+    new ones) a token sees all, or with a window what that and the sinks leave of
+    it for the end of its path, which stands as many places behind the context as
+    it has bits.  64 words must cover max_new."""
+    what = "attention_tree4"
+    if tree.dim() != 2 or tree.shape[0] != q.shape[0] or not tree.shape[1]:
+        raise ValueError(f"{what}: tree int64 [{q.shape[0]}, words], not {tuple(tree.shape)}")
+    _plain(what, "tree", tree, torch.int64, tree.shape, cache.device)
+    return _attention4(what, q, cache, page_table, lens, scale, starts, max_new, max_len, True, window,
+                       sinks, tree, lse, out)
+
+
+def _attention4(what, q, cache, page_table, lens, scale, starts, max_new, max_len, causal, window,
+                sinks, tree, lse, out):
     d = _dtype4(q, what)
     if q.dim() != 3:
         raise ValueError(f"{what}: q [tokens, heads, dh]")
@@ -814,15 +846,222 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
         _writable(what, "out", out, None if same else q, "q")
     sums = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if lse else None
     max_new, max_len, window = (min(int(n), 0x7fffffff) for n in (max_new, max_len, window))
-    if min(max_new, max_len, window) < 0:
-        raise ValueError(f"{what}: negative max_new, max_len or window")
+    if min(max_new, max_len, window) < 0 or sinks < 0:
+        raise ValueError(f"{what}: negative max_new, max_len, window or sinks")
+    words = 0 if tree is None else tree.shape[1]
+    if words and 64 * words < max_new:
+        raise ValueError(f"{what}: {words} words of 64 bits a token for up to {max_new} new tokens")
+    mask = None
+    if words or (sinks and window):
+        mask = _lib.Attn4Mask(min(int(sinks), 0x7fffffff), None if tree is None else tree.data_ptr(), words)
     causal = int(bool(causal))
     size = _workspace4(cache.pages, cache.page_size, cache.heads, dh, d, heads, tokens, batch, pages,
-                       max_new, max_len, causal, window, None if at is None else 256)
+                       max_new, max_len, causal, window, None if at is None else 256,
+                       *(() if mask is None else (mask.sinks, words)))
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     a = _lib.Attn4(q.data_ptr(), out.data_ptr(), None if sums is None else sums.data_ptr(), *qs, *os,
                    tokens, batch, page_table.data_ptr(), page_table.stride(0), pages,
                    lens.data_ptr(), at, d, heads, max_new, max_len, scale, causal, window,
                    None if work is None else work.data_ptr(), size)
-    _enqueue(cache._index, _lib.load().qph_attention_cache4, cache._ref, ctypes.byref(a))
+    if mask is None:
+        _enqueue(cache._index, _lib.load().qph_attention_cache4, cache._ref, ctypes.byref(a))
+    else:
+        _enqueue(cache._index, _lib.load().qph_attention_mask4, cache._ref, ctypes.byref(a),
+                 ctypes.byref(mask))
     return (out, sums) if lse else out
+
+
+# ------------------------------------------- a step that checks drafted tokens
+
+Step4 = collections.namedtuple("Step4", "starts lens slots positions ends tree")
+Step4.__doc__ = """What cache4_extend makes of a step: starts int32 [batch + 1], lens int32 [batch],
+slots int64 [tokens], positions int32 [tokens], ends int64 [2], tree int64 [tokens, words] or None."""
+
+
+def cache4_extend(page_table, lens, news, page_size, ring, ends, tokens, parents=None, max_new=None):
+    """Pages, slots, positions and masks of a step from its lengths, as a Step4; all on
+    the device, nothing waits.
+
+    Sequence b has lens[b] cached tokens (int32 [batch]) on the pages of its row of
+    page_table (int32 [batch, pages]) and grows by news[b] tokens (int32 [batch]), or
+    shrinks by -news[b].  Free pages are ring[i % len(ring)] (int32) for ends[0] <= i <
+    ends[1] (int64 [2]); a ring with room for every page of the pool never runs over.
+    page_table and the ring are written in place: pages that sequences take, in their
+    order, and pages that they give back, which the next call can take.  The entries
+    behind a sequence's last page mean nothing.
+
+    Of the step's rows, `tokens` in all, sequence b has starts[b] to starts[b + 1]: their
+    slots (for cache4_write) and positions (for rotary).  lens and ends are those after
+    the step.  A sequence whose pages are not all there, that its row of the table does
+    not hold or whose rows end past `tokens` is not granted: its length stays and its
+    slots are -1.  With parents, int32 [tokens], the new tokens are drafted trees:
+    parents[t] is the index of a row's parent among its sequence's new ones, smaller
+    than its own (else the context's), positions go by depth, and tree has
+    attention_tree4's masks for up to max_new (needed then) new tokens a sequence."""
+    what = "cache4_extend"
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (
+            page_table.stride(1) != 1 and page_table.shape[1] > 1 and page_table.numel()):
+        raise ValueError(f"{what}: page_table int32 [batch, pages], rows contiguous")
+    dev = page_table.device
+    _on(what, dev, "page_table", page_table)
+    batch, pages = page_table.shape
+    _plain(what, "lens", lens, torch.int32, (batch,), dev)
+    _plain(what, "news", news, torch.int32, (batch,), dev)
+    _plain(what, "ends", ends, torch.int64, (2,), dev)
+    if ring.dim() != 1 or not ring.shape[0]:
+        raise ValueError(f"{what}: ring int32 [pages of the pool]")
+    _plain(what, "ring", ring, torch.int32, ring.shape, dev)
+    if tokens < 0:
+        raise ValueError(f"{what}: negative tokens")
+    _writable(what, "page_table", page_table)
+    inputs = [("page_table", page_table), ("ring", ring), ("lens", lens), ("news", news), ("ends", ends)]
+    tree, words = None, 0
+    if parents is not None:
+        if max_new is None or max_new < 1:
+            raise ValueError(f"{what}: parents need max_new")
+        _plain(what, "parents", parents, torch.int32, (tokens,), dev)
+        inputs.append(("parents", parents))
+        words = (int(max_new) + 63) // 64
+        tree = torch.empty((tokens, words), dtype=torch.int64, device=dev)
+    for i in (0, 1):
+        for name, t in inputs[i + 1:]:
+            _apart(what, inputs[i][0], inputs[i][1], name, t)
+    starts = torch.empty(batch + 1, dtype=torch.int32, device=dev)
+    after = torch.empty(batch, dtype=torch.int32, device=dev)
+    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+    positions = torch.empty(tokens, dtype=torch.int32, device=dev)
+    left = torch.empty(2, dtype=torch.int64, device=dev)
+    size = _workspace_extend(batch)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    a = _lib.Extend4(page_table.data_ptr(), page_table.stride(0), pages, batch, lens.data_ptr(),
+                     news.data_ptr(), ring.data_ptr(), ring.shape[0], ends.data_ptr(), tokens,
+                     None if parents is None else parents.data_ptr(), words, starts.data_ptr(),
+                     after.data_ptr(), slots.data_ptr(), positions.data_ptr(), left.data_ptr(),
+                     None if tree is None else tree.data_ptr(), page_size,
+                     None if work is None else work.data_ptr(), size)
+    _enqueue(dev.index, _lib.load().qph_cache4_extend, ctypes.byref(a))
+    return Step4(starts, after, slots, positions, left, tree)
+
+
+def _apart(what, name, t, other_name, other):
+    """Refuses two tensors whose memory, from end to end, overlaps."""
+    def span(x):
+        at = x.data_ptr()
+        return at, at + x.element_size() * (1 + sum(st * (n - 1) for st, n in zip(x.stride(), x.shape)))
+    if t.numel() and other.numel():
+        (a, b), (c, d) = span(t), span(other)
+        if a < d and c < b:
+            raise ValueError(f"{what}: {name} and {other_name} share memory")
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_extend(batch):
+    size = ctypes.c_size_t()
+    check(_lib.load().qph_cache4_extend_workspace(batch, ctypes.byref(size)))
+    return size.value
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_move(pages, page, heads, dh, tokens):
+    """qph_cache4_move_workspace, which sees the sizes alone."""
+    c, size = _lib.Cache4(256, 256, 256, 256, pages, page, heads, dh), ctypes.c_size_t()
+    check(_lib.load().qph_cache4_move_workspace(ctypes.byref(c), tokens, ctypes.byref(size)))
+    return size.value
+
+
+def cache4_move(cache, src, dst):
+    """Tokens' keys and values from the slots src to the slots dst (int64 [tokens]
+    either), as they are held.  All are read before any is written, so that a slot may
+    be left and taken in one call.  A pair with a slot outside the pool is skipped; the
+    dst must differ."""
+    what = "cache4_move"
+    if src.dim() != 1:
+        raise ValueError(f"{what}: src [tokens]")
+    n = src.shape[0]
+    _plain(what, "src", src, torch.int64, (n,), cache.device)
+    _plain(what, "dst", dst, torch.int64, (n,), cache.device)
+    size = _workspace_move(cache.pages, cache.page_size, cache.heads, cache.dh, n)
+    work = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
+    _enqueue(cache._index, _lib.load().qph_cache4_move, cache._ref, src.data_ptr(), dst.data_ptr(), n,
+             None if work is None else work.data_ptr(), size)
+
+
+class Rotary(_Fixed):
+    """Which elements of a head of dh a rotation pairs, and how fast each pair turns:
+    turns int64 [pairs] in 2^-64ths of a turn a position (modulo one), axes int32
+    [pairs], the axis of positions that each goes by (0 to n_axes - 1).  Pair i is the
+    elements i and pairs + i, with neighbours 2 i and 2 i + 1; elements from 2 pairs on
+    stay.  rotary_plan makes one from frequencies; the two tensors' contents may change,
+    the tensors may not be replaced or moved."""
+    _parts = "dh", "turns", "axes", "n_axes", "neighbours"
+
+    def __init__(self, dh, turns, axes, n_axes, neighbours=False):
+        pairs = turns.shape[0] if turns.dim() == 1 else 0
+        if not 0 < pairs <= dh // 2 or n_axes < 1:
+            raise ValueError(f"Rotary: turns [pairs] of 1 to {dh // 2} pairs, on one axis or more")
+        _plain("Rotary", "turns", turns, torch.int64, (pairs,), turns.device)
+        _plain("Rotary", "axes", axes, torch.int32, (pairs,), turns.device)
+        self._fix(dh=int(dh), turns=turns, axes=axes, n_axes=int(n_axes), neighbours=bool(neighbours),
+                  pairs=pairs, device=turns.device, _index=turns.device.index,
+                  _ptrs=(turns.data_ptr(), axes.data_ptr()))
+
+
+_TWO_PI = fractions.Fraction(628318530717958647692528676655900576839433879875021, 10 ** 50)
+
+
+def rotary_plan(dh, freqs, axes=None, neighbours=False, device="cuda"):
+    """The Rotary of heads of dh elements whose pair i turns by freqs[i] radians a
+    position (numbers; usually base^(-i / pairs)) of axis axes[i] (default: 0)."""
+    freqs = [float(f) for f in freqs]
+    axes = [0] * len(freqs) if axes is None else [int(a) for a in axes]
+    if len(axes) != len(freqs) or not freqs or 2 * len(freqs) > dh:
+        raise ValueError(f"rotary_plan: {len(freqs)} frequencies and {len(axes)} axes for heads of {dh}")
+    if not all(math.isfinite(f) for f in freqs) or min(axes) < 0:
+        raise ValueError("rotary_plan: frequencies must be finite, axes not negative")
+    # (whole numbers: a float64 would hold 53 of the 64 bits)
+    turns = [round(fractions.Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in freqs]
+    turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in turns]
+    return Rotary(dh, torch.tensor(turns, dtype=torch.int64, device=device),
+                  torch.tensor(axes, dtype=torch.int32, device=device), max(axes) + 1, neighbours)
+
+
+def rotary(x, positions, plan, inverse=False, out=None):
+    """x [tokens, heads, dh] (float32, float16, bfloat16; tokens and heads of any strides)
+    with the pairs of a Rotary turned by their positions, int32 or int64 [tokens] (one
+    for every axis) or [axes, tokens], of any strides.  inverse turns back (the
+    rotation of a gradient too).  out may be x itself, and shares no memory with it
+    otherwise, nor its elements any."""
+    what = "rotary"
+    d = _dtype4(x, what)
+    if x.dim() != 3 or x.shape[2] != plan.dh:
+        raise ValueError(f"{what}: x [tokens, heads, {plan.dh}], not {tuple(x.shape)}")
+    tokens, heads, dh = x.shape
+    dev = plan.device
+    xs = _rows4(what, "x", x, plan, tokens, heads)
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: positions are {positions.dtype}, not int32 or int64")
+    if positions.dim() == 2 and positions.shape == (plan.n_axes, tokens):
+        ps = positions.stride()
+    elif positions.shape == (tokens,):
+        ps = 0, positions.stride(0)
+    else:
+        raise ValueError(f"{what}: positions [{tokens}] or [{plan.n_axes}, {tokens}], not "
+                         f"{tuple(positions.shape)}")
+    _on(what, dev, "positions", positions)
+    _no_grad(what, x, out)
+    if out is None:
+        out = x.new_empty((tokens, heads, dh))
+        os = out.stride()[:2]
+    else:
+        if out.dtype != x.dtype:
+            raise ValueError(f"{what}: out is {out.dtype}, x {x.dtype}")
+        os = _rows4(what, "out", out, plan, tokens, heads)
+        same = out.data_ptr() == x.data_ptr() and os == xs
+        _writable(what, "out", out, None if same else x, "x")
+        _apart(what, "out", out, "positions", positions)
+    turns, axes = plan._ptrs
+    a = _lib.RotaryArgs(x.data_ptr(), out.data_ptr(), *xs, *os, tokens, positions.data_ptr(), *ps, turns,
+                        axes, d, heads, dh, plan.pairs, plan.n_axes, positions.dtype == torch.int64,
+                        plan.neighbours, bool(inverse))
+    _enqueue(plan._index, _lib.load().qph_rotary, ctypes.byref(a))
+    return out
