@@ -432,7 +432,10 @@ QPH_API int qph_attention_cache4(qph_ctx* ctx, const qph_cache4* cache, const qp
  * context as the path is long).  A window hides no drafted token, causal is not
  * used, and bits from n on count for nothing.  tree_words is 0 without a tree and
  * max_new / 64 rounded up at least with one (drafted tokens past the words are not
- * seen).  Everything else is as in qph_attention_cache4, the workspace's rules too. */
+ * seen).  Where a head has many rows, the probabilities of bfloat16 rows keep 11
+ * bits before they meet the values, those of the others 21 and more.  The scales
+ * are 4-byte aligned.  Everything else is as in qph_attention_cache4, the
+ * workspace's rules too. */
 typedef struct {
   int64_t sinks;
   const uint64_t* tree;       /* [tokens][tree_words], device */

@@ -11,6 +11,73 @@ int launch_mask4_bf16(const Mask4& g, const Mask4Plan& p, int dh, hipStream_t s)
   return launch_mask4<BF16>(g, p, dh, s);
 }
 
+// Joins the splits of a row: dh / 4 lanes a row, four elements each, as many rows a wave as
+// its lanes hold.  A lane takes the splits' maxima and sums one after the other, then their
+// elements, eight in flight.
+template <typename E>
+__global__ __launch_bounds__(256) void mask4_join_kernel(Attn4 a, int dh, int each) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = dh / 4, sub = lane / per, at = lane - sub * per;
+  const int qheads = a.heads * a.group;
+  const int64_t all = a.tokens * qheads;
+  const float c = fabsf(a.scale) * kLog2e;
+  for (int64_t row = ((int64_t)blockIdx.x * 4 + wave) * each + sub; row - sub < all;
+       row += (int64_t)gridDim.x * 4 * each) {
+    const int64_t t = row / qheads;
+    if (sub >= each || row >= all) continue;
+    if (a.starts && (t < a.starts[0] || t >= a.starts[a.batch])) continue;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; s++) top = fmaxf(top, a.part_ml[2 * (s * all + row)]);
+    float sum = 0.0f;
+    bool some = false;
+    f32x4 v = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < a.splits; s0 += 8) {
+      f32x4 u[8];
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int64_t part = (int64_t)min(s0 + i, a.splits - 1) * all + row;
+        const float m = a.part_ml[2 * part], l = a.part_ml[2 * part + 1];
+        // (splits without keys have stored nothing)
+        const bool there = s0 + i < a.splits && l != 0.0f;
+        w[i] = there ? exp2_(rescale(m, top, c)) : 0.0f;
+        sum += there ? w[i] * l : 0.0f;
+        some |= there;
+        u[i] = f32x4{0, 0, 0, 0};
+        if (there) u[i] = *(const f32x4*)(a.part_o + part * dh + 4 * at);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += w[i] * u[i][e];
+    }
+    if (a.lse && at == 0) a.lse[row] = some ? log_sum(top, sum, fabsf(a.scale)) : -INFINITY;
+    const float inv = some ? 1.0f / sum : 0.0f;
+    typename E::type y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = (typename E::type)(v[e] * inv);
+    __builtin_memcpy((typename E::type*)a.out + t * a.ot + (row % qheads) * a.oh + 4 * at, y, sizeof y);
+  }
+}
+
+template <typename E>
+static int launch_mask4_join(const Attn4& a, int dh, hipStream_t s) {
+  const int each = 64 / (dh / 4);
+  const int64_t rows = a.tokens * a.heads * a.group;
+  const dim3 grid((unsigned)std::min<int64_t>((rows + 4 * each - 1) / (4 * each), 1 << 20));
+  hipLaunchKernelGGL(mask4_join_kernel<E>, grid, dim3(256), 0, s, a, dh, each);
+  return launch_check("mask4_join_kernel");
+}
+
+// How a call is split.  Up to 32 rows of a sequence and head take the few-row form.  Up to
+// 256 take it too while its workgroups all run at once and read little of the cache between
+// them: each decodes the keys of its 32 rows anew, which costs less than the many-row form's
+// longer way to its first product.  (32 query heads over 8; few-row against many-row form:
+// one sequence, 256 rows of 130 bfloat16 keys 13 and 22 us, of 4000 keys 36 and 47, of 16000
+// 74 and 58; eight sequences, 128 rows of 4000 keys 62 and 48; 24 sequences, 256 rows of 130
+// keys 53 and 24, 96 rows 21 and 20.  In float32, whose products
+// cost more than the decoding: eight sequences, 40 rows of 16000 keys 88 and 110 us, 128
+// rows 192 and 158.)
 static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_attn4_mask* mask) {
   Mask4Plan r{};
   const int64_t rows = std::min<int64_t>((int64_t)p->max_new * (p->heads / c->heads), 1 << 30);
@@ -18,17 +85,32 @@ static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_a
                                                                          std::min(mask->sinks, kMaxKeys))
                                      : p->max_len;
   const int64_t seqs = (int64_t)p->batch * c->heads;
-  r.shared = rows > 32;
-  r.nq = rows > 16 ? 2 : 1;
-  const int64_t tiles = (rows + mask4_rows(r.nq, r.shared) - 1) / mask4_rows(r.nq, r.shared);
+  const int terms = p->dtype == QPH_F32 ? 3 : 1, w = c->dh / 32;
+  r.nq = rows > 16 ? mask4_nq(terms, w) : 1;
+  int64_t tiles = (rows + 16 * r.nq - 1) / (16 * r.nq);
+  const bool few = rows <= 32 || (rows <= 256 && tiles * seqs <= 768 &&
+                                  tiles * seqs * keys <= (terms > 1 ? 1000000 : 400000));
+  if (!few) {
+    const int64_t most = mask4_waves(terms, w);
+    const int64_t groups = (tiles + most - 1) / most;
+    r.waves = (int)std::max<int64_t>((tiles + groups - 1) / groups, 4);
+    tiles = groups;
+  }
   // (as in attn4_plan: past a million workgroups in all they take further tiles in turn)
   r.row_tiles = (int)std::clamp<int64_t>(tiles, 1, std::max<int64_t>(1, ((int64_t)1 << 20) / seqs));
   r.splits = 1;
   r.chunk = (int64_t)1 << 40;
-  const int64_t blocks = r.row_tiles * seqs, most = r.shared ? 1024 : 1536;
+  const int64_t blocks = r.row_tiles * seqs;
+  // Keys are split until the workgroups fill the chip: three to a CU in the few-row form; in
+  // the many-row form one of more than four waves, or of four waves two, and four where
+  // sequences of several lengths make some end early.  A split has 512 keys at least, 256
+  // where that leaves CUs idle.
+  const int64_t most = !r.waves ? 768 : (r.waves > 4 ? 256 : (p->batch > 1 ? 1024 : 512));
   const int64_t least = keys / 512 >= (255 + blocks) / blocks ? 512 : 256;
-  if (2 * blocks <= most && keys > 2 * least) {
-    int64_t n = std::min<int64_t>({most / blocks, (keys + least - 1) / least, 64});
+  int64_t n = 1;
+  if (2 * blocks <= most && keys > 2 * least)
+    n = std::min<int64_t>({most / blocks, (keys + least - 1) / least, 64});
+  if (n > 1) {
     r.chunk = ((keys + n - 1) / n + 127) / 128 * 128;
     n = (keys + r.chunk - 1) / r.chunk;
     if (n > 1) r.splits = (int)n;
@@ -80,6 +162,8 @@ QPH_API int qph_attention_mask4(qph_ctx* ctx, const qph_cache4* cache, const qph
                                 " bytes, needs " + std::to_string(p.workspace));
   if ((uintptr_t)args->workspace % 16)
     return fail(QPH_EINVAL, "attention_mask4: workspace is not 16-byte aligned");
+  if (((uintptr_t)cache->k_scales | (uintptr_t)cache->v_scales) % 4)
+    return fail(QPH_EINVAL, "attention_mask4: scales are not 4-byte aligned");
   if ((int64_t)p.row_tiles * p.splits * cache->heads * args->batch > kMaxGroups)
     return fail(QPH_EUNSUPPORTED, "attention_mask4: batch too large for one call");
   if (!ctx) return fail(QPH_EINVAL, "null context");
@@ -103,7 +187,14 @@ QPH_API int qph_attention_mask4(qph_ctx* ctx, const qph_cache4* cache, const qph
   else if (args->dtype == QPH_F16) rc = launch_mask4_f16(g, p, cache->dh, ctx->stream);
   else rc = launch_mask4_bf16(g, p, cache->dh, ctx->stream);
   QPH_TRY(rc);
-  return attn4_join(g.a, args->dtype, cache->dh, ctx->stream);
+  // Joined by attn4_join where splits are many and rows few (its workgroups share a row's
+  // splits), else with several rows a wave.
+  if (p.splits == 1) return QPH_OK;
+  if (p.splits > 8 && args->tokens * args->heads < 4096)
+    return attn4_join(g.a, args->dtype, cache->dh, ctx->stream);
+  if (args->dtype == QPH_F32) return launch_mask4_join<F32>(g.a, cache->dh, ctx->stream);
+  if (args->dtype == QPH_F16) return launch_mask4_join<F16>(g.a, cache->dh, ctx->stream);
+  return launch_mask4_join<BF16>(g.a, cache->dh, ctx->stream);
 }
 
 }  // extern "C"

@@ -845,7 +845,8 @@ def _attention4(what, q, cache, page_table, lens, scale, starts, max_new, max_le
         same = out.data_ptr() == q.data_ptr() and os == qs
         _writable(what, "out", out, None if same else q, "q")
     sums = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if lse else None
-    max_new, max_len, window = (min(int(n), 0x7fffffff) for n in (max_new, max_len, window))
+    max_new, max_len = min(int(max_new), 0x7fffffff), min(int(max_len), 0x7fffffff)
+    window = min(int(window), 0x7fffffff)
     if min(max_new, max_len, window) < 0 or sinks < 0:
         raise ValueError(f"{what}: negative max_new, max_len, window or sinks")
     words = 0 if tree is None else tree.shape[1]
@@ -913,19 +914,25 @@ def cache4_extend(page_table, lens, news, page_size, ring, ends, tokens, parents
     _plain(what, "ring", ring, torch.int32, ring.shape, dev)
     if tokens < 0:
         raise ValueError(f"{what}: negative tokens")
-    _writable(what, "page_table", page_table)
-    inputs = [("page_table", page_table), ("ring", ring), ("lens", lens), ("news", news), ("ends", ends)]
+    stride = page_table.stride(0)
+    if batch > 1 and stride < pages:
+        raise ValueError(f"{what}: page_table of strides {page_table.stride()} overlaps itself")
+    inputs = [("page_table", page_table, 4 * (stride * max(batch - 1, 0) + pages)), ("ring", ring, 4 * ring.shape[0]),
+              ("lens", lens, 4 * batch), ("news", news, 4 * batch), ("ends", ends, 16)]
     tree, words = None, 0
     if parents is not None:
         if max_new is None or max_new < 1:
             raise ValueError(f"{what}: parents need max_new")
         _plain(what, "parents", parents, torch.int32, (tokens,), dev)
-        inputs.append(("parents", parents))
+        inputs.append(("parents", parents, 4 * tokens))
         words = (int(max_new) + 63) // 64
         tree = torch.empty((tokens, words), dtype=torch.int64, device=dev)
-    for i in (0, 1):
-        for name, t in inputs[i + 1:]:
-            _apart(what, inputs[i][0], inputs[i][1], name, t)
+    # the two that are written lie apart from each other and from all that is read
+    spans = [(t.data_ptr(), size) for _, t, size in inputs]
+    for i, (at, size) in enumerate(spans[:2]):
+        for j, (other, length) in enumerate(spans[i + 1:]):
+            if at < other + length and other < at + size and size and length:
+                raise ValueError(f"{what}: {inputs[i][0]} and {inputs[i + 1 + j][0]} share memory")
     starts = torch.empty(batch + 1, dtype=torch.int32, device=dev)
     after = torch.empty(batch, dtype=torch.int32, device=dev)
     slots = torch.empty(tokens, dtype=torch.int64, device=dev)
@@ -933,7 +940,7 @@ def cache4_extend(page_table, lens, news, page_size, ring, ends, tokens, parents
     left = torch.empty(2, dtype=torch.int64, device=dev)
     size = _workspace_extend(batch)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    a = _lib.Extend4(page_table.data_ptr(), page_table.stride(0), pages, batch, lens.data_ptr(),
+    a = _lib.Extend4(spans[0][0], stride, pages, batch, lens.data_ptr(),
                      news.data_ptr(), ring.data_ptr(), ring.shape[0], ends.data_ptr(), tokens,
                      None if parents is None else parents.data_ptr(), words, starts.data_ptr(),
                      after.data_ptr(), slots.data_ptr(), positions.data_ptr(), left.data_ptr(),
@@ -941,17 +948,6 @@ def cache4_extend(page_table, lens, news, page_size, ring, ends, tokens, parents
                      None if work is None else work.data_ptr(), size)
     _enqueue(dev.index, _lib.load().qph_cache4_extend, ctypes.byref(a))
     return Step4(starts, after, slots, positions, left, tree)
-
-
-def _apart(what, name, t, other_name, other):
-    """Refuses two tensors whose memory, from end to end, overlaps."""
-    def span(x):
-        at = x.data_ptr()
-        return at, at + x.element_size() * (1 + sum(st * (n - 1) for st, n in zip(x.stride(), x.shape)))
-    if t.numel() and other.numel():
-        (a, b), (c, d) = span(t), span(other)
-        if a < d and c < b:
-            raise ValueError(f"{what}: {name} and {other_name} share memory")
 
 
 @functools.lru_cache(maxsize=256)
@@ -1058,7 +1054,7 @@ def rotary(x, positions, plan, inverse=False, out=None):
         os = _rows4(what, "out", out, plan, tokens, heads)
         same = out.data_ptr() == x.data_ptr() and os == xs
         _writable(what, "out", out, None if same else x, "x")
-        _apart(what, "out", out, "positions", positions)
+        _writable(what, "out", out, positions, "positions")
     turns, axes = plan._ptrs
     a = _lib.RotaryArgs(x.data_ptr(), out.data_ptr(), *xs, *os, tokens, positions.data_ptr(), *ps, turns,
                         axes, d, heads, dh, plan.pairs, plan.n_axes, positions.dtype == torch.int64,

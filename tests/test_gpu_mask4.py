@@ -91,11 +91,23 @@ def check(torch, c, q, table, lens, news, window=0, sinks=0, trees=None, causal=
                 continue
             see = there & visible(n, news[b], i, causal, window, sinks, None if trees is None else trees[b])
             row = starts[b] + i
-            want, tol, (lse, ltol) = attend_row(qd[row], k[pg[see], pos[see] % page],
-                                                v[pg[see], pos[see] % page], scale, terms, group)
+            want, tol, (lse, ltol) = attend(qd[row], k[pg[see], pos[see] % page],
+                                            v[pg[see], pos[see] % page], scale, terms, group)
             close(y[row], want, tol + half_step(torch, q.dtype, want) * 1.001, f"{name}: row {row} ({b}, {i})")
             close(sums[row], lse, ltol, f"{name}: lse of row {row}")
     return y, sums
+
+
+def attend(q, k, v, scale, terms, group):
+    """attend_row; a bfloat16 row's probabilities may be held as float16, each off by half a
+    step of it, 2^-11 of itself, which the values pass on."""
+    out, tol, sums = attend_row(q, k, v, scale, terms, group)
+    for h in range(q.shape[0] if terms == 1 and k.shape[0] else 0):
+        s = k[:, h // group] @ q[h] * scale
+        p = np.exp(s - s.max())
+        with np.errstate(invalid="ignore"):
+            tol[h] += 2.0 ** -11 * (p / p.sum() @ np.abs(v[:, h // group]))
+    return out, tol, sums
 
 
 def queries(torch, rng, tokens, heads, dh, dtype):

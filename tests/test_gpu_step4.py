@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from test_gpu_decode4 import DTYPES, HEAD_DIMS, close, half_step, host, make_cache, numbers
-from test_gpu_mask4 import attend_row, drafted, paths, words_of
+from test_gpu_mask4 import attend, drafted, paths, words_of
 
 pytestmark = pytest.mark.gpu
 
@@ -516,7 +516,7 @@ def test_steps_that_check_drafted_trees(gpu, dtype):
             pg = tab[b, pos // page]
             for i in range(news[b]):
                 vis = (pos < host_lens[b]) | np.concatenate([np.zeros(host_lens[b], bool), see[i]])
-                want, tol, (lse, ltol) = attend_row(host(q[st[b] + i]), kd[pg[vis], pos[vis] % page],
+                want, tol, (lse, ltol) = attend(host(q[st[b] + i]), kd[pg[vis], pos[vis] % page],
                                                     vd[pg[vis], pos[vis] % page], dh ** -0.5, terms, group)
                 close(host(y[st[b] + i]), want, tol + half_step(gpu, t, want) * 1.001, f"step {step} row {b} {i}")
                 close(host(sums[st[b] + i]), lse, ltol, f"step {step} sum {b} {i}")

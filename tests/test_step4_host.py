@@ -62,6 +62,10 @@ def test_attention_arguments(lib):  # noqa: F811
     refused(lib, call(mask(tree=None)), EINVAL, "NULL argument")
     refused(lib, call(mask(tree=None, tree_words=0)), EINVAL, "null context")
     refused(lib, call(workspace=A + 4), EINVAL, "16-byte")
+    for part in ("k_scales", "v_scales"):
+        odd = cache(**{part: A + 2})
+        refused(lib, lib.qph_attention_mask4(None, ctypes.byref(odd), ctypes.byref(attn()), ctypes.byref(mask())),
+                EINVAL, "scales are not 4-byte aligned")
     refused(lib, call(), EINVAL, "null context")
     refused(lib, call(tokens=0, batch=0, q=None, out=None, lens=None), EINVAL, "null context")
     # a call that is split needs its workspace
