@@ -511,13 +511,20 @@ __device__ __forceinline__ void store_rows(const Attn4& a, const Walk4& w, const
 
 // ------------------------------------------------------------- few rows
 
+// Waves of a workgroup: four, and up to twelve where registers leave room for three a SIMD
+// (a longer row of waves in place of workgroups that split the keys saves their join).
+template <int NQ>
+constexpr int mask4_few_waves(int terms, int w) { return NQ == 1 && w <= 4 && terms < 3 ? 12 : 4; }
+
 template <typename E, int W, int NQ>
-__global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) void mask4_few_kernel(Mask4 g) {
+__global__ __launch_bounds__(64 * mask4_few_waves<NQ>(E::terms, W), mask4_few_waves<NQ>(E::terms, W) / 4) void
+mask4_few_kernel(Mask4 g) {
   const Attn4& a = g.a;
   constexpr int R = 16 * NQ;
   extern __shared__ u32x4 lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, kg = lane >> 4;
+  const int waves = mask4_few_waves<NQ>(E::terms, W) > 4 ? blockDim.x >> 6 : 4;
   Walk4 w(g);
   const Place<W> place(li, kg);
   for (int64_t tile = w.rt0; tile * R < w.rows; tile += a.row_tiles) {
@@ -530,7 +537,7 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
 #pragma unroll
     for (int q = 0; q < NQ; q++) shift[q] = 0.0f;
 
-    // This wave's tiles t, t + 4, ...; the next one's loads in flight while one is computed
+    // This wave's tiles t, t + waves, ...; the next one's loads in flight while one is computed
     // (with more rows a wave the values' come late, behind the keys' products).
     int t = wave;
     if (t < w.tiles) {
@@ -541,34 +548,34 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
       Pages pa = find_pages(a, page_ids(a, w.table, j0, w.ghi), j0, w.h), pb;
       load_keys<W>(a, pa, place, ka);
       if (!late) load_values<W>(a, pa, place, va);
-      int j1 = w.key_of(min(t + 4, w.tiles - 1));
+      int j1 = w.key_of(min(t + waves, w.tiles - 1));
       PageIds ids = page_ids(a, w.table, j1, w.ghi);
       while (true) {
         if (late) load_values<W>(a, pa, place, va);
         pb = find_pages(a, ids, j1, w.h);
         load_keys<W>(a, pb, place, kb);
         if (!late) load_values<W>(a, pb, place, vb);
-        const int j2 = w.key_of(min(t + 8, w.tiles - 1));
+        const int j2 = w.key_of(min(t + 2 * waves, w.tiles - 1));
         ids = page_ids(a, w.table, j2, w.ghi);
         __builtin_amdgcn_sched_barrier(0);
         own_tile<E, W, NQ, false>(g, w, rows, qf, ka, va, pa, j0, li, kg, place, shift, sums);
-        t += 4;
+        t += waves;
         if (t >= w.tiles) break;
         if (late) load_values<W>(a, pb, place, va);
         pa = find_pages(a, ids, j2, w.h);
         load_keys<W>(a, pa, place, ka);
         if (!late) load_values<W>(a, pa, place, va);
-        j0 = w.key_of(min(t + 8, w.tiles - 1));
+        j0 = w.key_of(min(t + 2 * waves, w.tiles - 1));
         ids = page_ids(a, w.table, j0, w.ghi);
         __builtin_amdgcn_sched_barrier(0);
         own_tile<E, W, NQ, false>(g, w, rows, qf, kb, late ? va : vb, pb, j1, li, kg, place, shift, sums);
-        t += 4;
+        t += waves;
         if (t >= w.tiles) break;
         j1 = j0;
         j0 = j2;
       }
     }
-    if (sums.unsure()) walk_again<E, W, NQ>(g, w, rows, qf, wave, 4, li, kg, place, shift, sums);
+    if (sums.unsure()) walk_again<E, W, NQ>(g, w, rows, qf, wave, waves, li, kg, place, shift, sums);
     auto& o = sums.o;
     auto& m = sums.m;
     auto& l = sums.l;
@@ -579,8 +586,8 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
       m[q] += shift[q];
       l[q] = column_sum(l[q]);
     }
-    float* ml = (float*)lds;                  // [4][NQ * 16][2]
-    float* ol = ml + 4 * NQ * 32;             // [4 waves][NQ * 2W * 4][64]
+    float* ml = (float*)lds;                  // [waves][NQ * 16][2]
+    float* ol = ml + waves * NQ * 32;         // [waves][NQ * 2W * 4][64]
     __syncthreads();                          // (an earlier tile's reads)
     if (kg == 0) {
 #pragma unroll
@@ -597,29 +604,24 @@ __global__ __launch_bounds__(256, NQ == 1 && W <= 4 && E::terms < 3 ? 3 : 1) voi
         for (int r = 0; r < 4; r++)
           ol[((wave * NQ + q) * 8 * W + r * 2 * W + x) * 64 + lane] = o[q][x][r];
     __syncthreads();
+    if (wave > 3) continue;
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
-      float wm[4], top = -INFINITY, sum = 0.0f;
-#pragma unroll
-      for (int v = 0; v < 4; v++) {
-        wm[v] = ml[((v * NQ + q) * 16 + li) * 2];
-        top = fmaxf(top, wm[v]);
-      }
-#pragma unroll
-      for (int v = 0; v < 4; v++) {
-        wm[v] = top == -INFINITY ? 0.0f : exp2_(rescale(wm[v], top, sums.c));
-        sum += wm[v] * ml[((v * NQ + q) * 16 + li) * 2 + 1];
-      }
+      float top = -INFINITY;
+      for (int v = 0; v < waves; v++) top = fmaxf(top, ml[((v * NQ + q) * 16 + li) * 2]);
       m[q] = top;
-      l[q] = sum;
+      l[q] = 0.0f;
       // wave r takes the rows d = 2 W (4 kg + r) + x of every lane group
 #pragma unroll
-      for (int x = 0; x < 2 * W; x++) {
-        float f = 0.0f;
+      for (int x = 0; x < 2 * W; x++) o[q][x][0] = 0.0f;
+#pragma unroll 4
+      for (int v = 0; v < waves; v++) {
+        const float* from = ml + ((v * NQ + q) * 16 + li) * 2;
+        const float wm = top == -INFINITY ? 0.0f : exp2_(rescale(from[0], top, sums.c));
+        l[q] += wm * from[1];
 #pragma unroll
-        for (int v = 0; v < 4; v++)
-          f += wm[v] * ol[((v * NQ + q) * 8 * W + wave * 2 * W + x) * 64 + lane];
-        o[q][x][0] = f;
+        for (int x = 0; x < 2 * W; x++)
+          o[q][x][0] += wm * ol[((v * NQ + q) * 8 * W + wave * 2 * W + x) * 64 + lane];
       }
     }
     store_rows<E, W, NQ, 1>(a, w, rows, kg, wave, m, l, o);
@@ -956,7 +958,7 @@ mask4_shared_kernel(Mask4 g) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           p[e] = exp2_(__builtin_fmaf(s[i][e / 4][q][e % 4], sums.c, -mc[q]));
-          sum += p[e];
+          sum = e ? sum + p[e] : p[e];
         }
         sums.l[q] += sum;
         if constexpr (VH) {
@@ -1032,7 +1034,10 @@ mask4_shared_kernel(Mask4 g) {
           for (int e = 1; e < 16; e++) mx[q] = fmaxf(mx[q], s[e / 8][e / 4 % 2][q][e % 4]);
           grows |= mx[q] > sums.m[q];
         }
-        if (__any(grows)) {
+        // (all lanes or none; said as each lane's own choice, for which the compiler scales
+        // the sums where they are: else it copies all of them every round, 5% of the time)
+        const bool some = __any(grows);
+        if (grows | some) {
 #pragma unroll
           for (int q = 0; q < NQ; q++) sums.raise_to(q, column_max(mx[q]));
         }
@@ -1101,18 +1106,18 @@ mask4_shared_kernel(Mask4 g) {
 // How a call is run: waves of a workgroup that share tiles (0: few rows), column tiles
 // a wave.
 struct Mask4Plan {
-  int nq, waves;
+  int nq, waves, few;             // (few: waves that share few rows)
   int row_tiles, splits;
   int64_t chunk;
   size_t workspace;
 };
 
 template <typename E, int W, int NQ>
-static int launch_mask4_few(const Mask4& g, hipStream_t s) {
-  const size_t lds = (size_t)4 * NQ * (32 + 2 * W * 4 * 64) * 4;
+static int launch_mask4_few(const Mask4& g, int few, hipStream_t s) {
+  const size_t lds = (size_t)few * NQ * (32 + 2 * W * 4 * 64) * 4;
   if (lds > 65536) QPH_TRY(allow_full_lds((const void*)mask4_few_kernel<E, W, NQ>));
   const int64_t blocks = (int64_t)g.a.row_tiles * g.a.splits * g.a.heads * g.a.batch;
-  hipLaunchKernelGGL((mask4_few_kernel<E, W, NQ>), dim3((unsigned)blocks), dim3(256), lds, s, g);
+  hipLaunchKernelGGL((mask4_few_kernel<E, W, NQ>), dim3((unsigned)blocks), dim3(64 * few), lds, s, g);
   return launch_check("mask4_few_kernel");
 }
 
@@ -1129,9 +1134,9 @@ template <typename E, int W>
 static int launch_mask4_w(const Mask4& g, const Mask4Plan& p, hipStream_t s) {
   if (p.waves) return launch_mask4_shared<E, W, mask4_nq(E::terms, W)>(g, p.waves, s);
   if constexpr (mask4_nq(E::terms, W) == 2) {
-    if (p.nq == 2) return launch_mask4_few<E, W, 2>(g, s);
+    if (p.nq == 2) return launch_mask4_few<E, W, 2>(g, p.few, s);
   }
-  return launch_mask4_few<E, W, 1>(g, s);
+  return launch_mask4_few<E, W, 1>(g, p.few, s);
 }
 
 template <typename E>

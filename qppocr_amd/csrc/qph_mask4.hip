@@ -110,6 +110,11 @@ static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_a
   int64_t n = 1;
   if (2 * blocks <= most && keys > 2 * least)
     n = std::min<int64_t>({most / blocks, (keys + least - 1) / least, 64});
+  // Three splits of few rows where a CU has one workgroup: twelve waves of it instead, without
+  // a join (32 sequences of 8 heads, windows of 4096: 36.8 us, 40.0 with splits).  Two splits
+  // are kept: eight waves a workgroup leave some CUs two (40 sequences: 58 us, 47 with splits).
+  r.few = !r.waves && r.nq == 1 && n == 3 && blocks <= 256 ? mask4_few_waves<1>(terms, w) : 4;
+  if (r.few > 4) n = 1;
   if (n > 1) {
     r.chunk = ((keys + n - 1) / n + 127) / 128 * 128;
     n = (keys + r.chunk - 1) / r.chunk;
