@@ -31,6 +31,13 @@ struct Mask4 {
   int words;                      // of 32 bits
 };
 
+// What a workgroup works on: a sequence's head, from a row tile on, and of its keys (the two
+// runs counted as one) those from va to vb, which are split number `split` of them.
+struct Part4 {
+  int b, h, rt0, split;
+  int64_t va, vb;
+};
+
 // The four bits of a tree's row from drafted token d on (none before the first and past the
 // words).  Without branches, so that the loads of several go out together.
 __device__ __forceinline__ unsigned path_bits(const unsigned* row, int words, int d) {
@@ -55,18 +62,10 @@ struct Walk4 {
   int i0;                         // its first row's token,
   unsigned rem;                   // and query head of this cache head
 
-  __device__ __forceinline__ explicit Walk4(const Mask4& g) {
+  __device__ __forceinline__ Walk4(const Mask4& g, const Part4& part) {
     const Attn4& a = g.a;
-    // Neighbouring workgroups go to the card's eight dies in turn: heads are next to each
-    // other, so that the row tiles of one find its keys in their die's cache, and splits
-    // come last, so that those without keys (of shorter sequences) are no die's more than
-    // another's (32 ragged sequences of 8 heads, 8 splits: 454 us with splits next to each
-    // other, 154 so).
-    unsigned id = blockIdx.x;
-    h = id % a.heads; id /= a.heads;
-    const int b = id % a.batch; id /= a.batch;
-    rt0 = id % a.row_tiles;
-    split = id / a.row_tiles;
+    const int b = part.b;
+    h = part.h; rt0 = part.rt0; split = part.split;
     // inside what the caller's buffers hold whatever the device arrays say
     int64_t t1;
     if (a.starts) {
@@ -88,7 +87,7 @@ struct Walk4 {
     // (a path's end stands at first - 1 at least, which is that of no tokens)
     s32 = (min(sinks, len) + 31) & ~31;
     const int base = window > 0 ? max(s32, window_from((int64_t)first - tree) & ~31) : 0;
-    const int64_t va = split * a.chunk, vb = split == a.splits - 1 ? INT64_MAX / 2 : va + a.chunk;
+    const int64_t va = part.va, vb = part.vb;
     a0 = (int)min(va, (int64_t)s32); a1 = (int)min(vb, (int64_t)s32);
     bfrom = base + max(va - s32, (int64_t)0); bto = base + max(vb - s32, (int64_t)0);
   }
@@ -121,6 +120,107 @@ struct Walk4 {
 
   __device__ __forceinline__ int key_of(int t) const { return t < n1 ? a0 + 32 * t : b0 + 32 * (t - n1); }
 };
+
+// The part of a workgroup where all splits have as many keys.  Neighbouring workgroups go to
+// the card's eight dies in turn: heads are next to each other, so that the row tiles of one
+// find its keys in their die's cache, and splits come last, so that those without keys (of
+// shorter sequences) are no die's more than another's (32 ragged sequences of 8 heads, 8
+// splits: 454 us with splits next to each other, 154 so).
+__device__ __forceinline__ Part4 part_of_block(const Attn4& a) {
+  Part4 p;
+  unsigned id = blockIdx.x;
+  p.h = id % a.heads; id /= a.heads;
+  p.b = id % a.batch; id /= a.batch;
+  p.rt0 = id % a.row_tiles;
+  p.split = id / a.row_tiles;
+  p.va = p.split * a.chunk;
+  p.vb = p.split == a.splits - 1 ? INT64_MAX / 2 : p.va + a.chunk;
+  return p;
+}
+
+// In pairs of tiles: the least share, and what a part costs beside its own (its queries, the
+// first loads, its sums; 32 ragged sequences of 8 heads: 207 us counted as nothing, 151 as
+// 3, 135 as 6, 136 as 10).
+constexpr int64_t kLeastShare = 4;
+constexpr unsigned kPartCost = 6;
+
+
+// The next part of a workgroup's even share: of the pairs of tiles of all sequences and heads,
+// kPartCost places ahead of each and one after the other, those from `at` (-1: none yet) to
+// `end`.  Each lane counts a sequence's (at most 64); one whose rows see no keys has a pair all
+// the same, so that they are stored.  `parts` is the number of splits that the keys of the
+// part's sequence and head have in all.  False: none is left.
+__device__ __forceinline__ bool next_part(const Mask4& g, int64_t& at, int64_t& end, Part4& part, int& parts) {
+  const Attn4& a = g.a;
+  const int lane = threadIdx.x & 63;
+  unsigned mine = 0;
+  if (lane < a.batch) {
+    const Walk4 w(g, Part4{lane, 0, 0, 0, 0, INT64_MAX / 2});
+    const int hi = w.tree ? w.len : w.border((int64_t)w.first + w.news - 1);
+    const int64_t tiles = w.s32 / 32 + ((max((int64_t)hi - w.bfrom, (int64_t)0) + 31) >> 5);
+    mine = w.news ? max((unsigned)((tiles + 1) >> 1), 1u) + kPartCost : 0u;
+  }
+  unsigned upto = mine, most = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const unsigned before = __shfl_up(upto, d);
+    upto += lane >= d ? before : 0u;
+    most = max(most, (unsigned)__shfl_xor(most, d));
+  }
+  const unsigned n = a.heads;
+  const int64_t all = (int64_t)(unsigned)__builtin_amdgcn_readlane(upto, 63) * n;
+  most = __builtin_amdgcn_readfirstlane(most);
+  const int64_t share = max(max((all + gridDim.x - 1) / gridDim.x, (int64_t)(most + a.splits - 2) / (a.splits - 1)),
+                            kLeastShare);
+  if (at < 0) {
+    at = blockIdx.x * share;
+    end = min(at + share, all);
+  }
+  if (at >= end) return false;
+  const int64_t from = (int64_t)(upto - mine) * n;
+  part.b = __builtin_ctzll(__ballot(from <= at && at < (int64_t)upto * n));
+  unsigned len = __builtin_amdgcn_readlane(mine, part.b);
+  const int64_t first = (int64_t)__builtin_amdgcn_readlane(upto - mine, part.b) * n;
+  part.h = (int)((at - first) / len);
+  part.rt0 = 0;
+  const int64_t head = first + (int64_t)part.h * len + kPartCost;
+  len -= kPartCost;
+  at = max(at, head);
+  if (at >= end) return false;
+  const int64_t x0 = at - head, x1 = min((int64_t)len, x0 + (end - at));
+  const int64_t before = head / share;
+  part.split = (int)(blockIdx.x - before);
+  parts = (int)((head + len - 1) / share - before) + 1;
+  part.va = 64 * x0;
+  part.vb = x1 == len ? INT64_MAX / 2 : 64 * x1;
+  at += x1 - x0;
+  return true;
+}
+
+// (for scalar registers: the compiler does not see that all lanes have the same)
+__device__ __forceinline__ int64_t same_in_all(int64_t v) {
+  return (int64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)v) |
+         (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+}
+
+struct EvenState {
+  int64_t at, end;
+  Part4 part;
+};
+
+// Says of the splits from `parts` on that a sequence's rows have no keys in them.
+__device__ __forceinline__ void unused_splits(const Mask4& g, const Part4& part, int parts) {
+  const Attn4& a = g.a;
+  const Walk4 w(g, part);
+  const int qheads = a.heads * a.group;
+  for (int s = parts; s < a.splits; s++)
+    for (int64_t r = threadIdx.x; r < w.rows; r += blockDim.x) {
+      const int64_t t = r / a.group;
+      float* ml = a.part_ml + 2 * (s * a.tokens * qheads + (w.t0 + t) * qheads + part.h * a.group + (r - t * a.group));
+      ml[0] = -INFINITY;
+      ml[1] = 0.0f;
+    }
+}
 
 // The rows of a wave, 16 to a column tile, and what each sees.
 template <int NQ>
@@ -525,7 +625,7 @@ mask4_few_kernel(Mask4 g) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, kg = lane >> 4;
   const int waves = mask4_few_waves<NQ>(E::terms, W) > 4 ? blockDim.x >> 6 : 4;
-  Walk4 w(g);
+  Walk4 w(g, part_of_block(a));
   const Place<W> place(li, kg);
   for (int64_t tile = w.rt0; tile * R < w.rows; tile += a.row_tiles) {
     w.tiles_of(tile * R, min(w.rows, tile * R + R) - 1, a.group);
@@ -747,10 +847,13 @@ __device__ __forceinline__ void take_values(const unsigned char* raw, int li, in
 // careful walks alone, the first of which finds the maxima.  (A function of its own:
 // seldom, and it would take registers from the kernel.)
 template <typename E, int W, int NQ>
-__device__ __noinline__ void slow_rows(const Mask4* g, int64_t r0, int R) {
+__device__ __noinline__ void slow_rows(const Mask4* g, int b, int h, int rt0, int split, int64_t va, int64_t vb,
+                                       int64_t r0, int R) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, kg = lane >> 4;
-  Walk4 w(*g);
+  r0 = same_in_all(r0);
+  Walk4 w(*g, Part4{(int)same_in_all(b), (int)same_in_all(h), (int)same_in_all(rt0), (int)same_in_all(split),
+                    same_in_all(va), same_in_all(vb)});
   if (r0 + 16 * NQ * wave >= w.rows) return;
   const Place<W> place(li, kg);
   w.tiles_of(r0, min(w.rows, r0 + R) - 1, g->a.group);
@@ -785,7 +888,7 @@ __device__ __noinline__ void slow_rows(const Mask4* g, int64_t r0, int R) {
 // matrix unit has work while the exponentials of the other tile are taken); keys of the
 // pair after that and values of the next are turned; and the codes of one pair more
 // are on their way.
-template <typename E, int W, int NQ>
+template <typename E, int W, int NQ, bool EVEN>
 __global__ __launch_bounds__(64 * mask4_waves(E::terms, W), mask4_waves(E::terms, W) / 4) void
 mask4_shared_kernel(Mask4 g) {
   const Attn4& a = g.a;
@@ -794,319 +897,350 @@ mask4_shared_kernel(Mask4 g) {
   constexpr int kHalf = 2 * W * 64;                         // 16-byte words of a tile's keys or values
   extern __shared__ u32x4 lds[];                            // keys [2][2], values [2][2]
   int* flags = (int*)(lds + 8 * kHalf);                     // [4][2], or [waves]; 16 words
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int li = lane & 15, kg = lane >> 4;
   const int waves = blockDim.x >> 6;
   const int R = 16 * NQ * waves;
-  Walk4 w(g);
-  const int slot = wave >> 1;
-  const bool keys = !(wave & 1), maker = wave < 4;
-  bool again = false;
-  if ((int64_t)w.rt0 * R < w.rows) {
-    w.tiles_of((int64_t)w.rt0 * R, min(w.rows, (int64_t)w.rt0 * R + R) - 1, a.group);
-    const unsigned d0 = 16 * NQ * wave;
-    const bool idle = w.r0 + d0 >= w.rows;
-    const int pairs = (w.tiles + 1) >> 1;
-    const Rows4<NQ> rows(g, w, d0, li);
-    // queries: as they are, or (float32) in bfloat16 terms
-    bf16x8 qf[NQ][KT][W];
-    if constexpr (KH) {
-      const _Float16 sign = a.scale < 0.0f ? (_Float16)-1.0f : (_Float16)1.0f;
-#pragma unroll
-      for (int q = 0; q < NQ; q++)
-#pragma unroll
-        for (int n = 0; n < W; n++) {
-          f16x8 v;
-          __builtin_memcpy(&v, (const _Float16*)a.q + (w.t0 + rows.tok[q]) * a.qt + rows.head[q] * a.qh +
-                                   8 * (W * kg + n), 16);
-          qf[q][0][n] = __builtin_bit_cast(bf16x8, v * sign);
-        }
+  // (EVEN: what is left of the share and the part at hand, kept here: they would take
+  // registers that the walk needs)
+  EvenState* state = (EvenState*)(flags + 16);
+  if constexpr (EVEN) {
+    if (threadIdx.x == 0) state->at = -1;
+    __syncthreads();
+  }
+  while (true) {
+    // (what follows from the lane is found anew each time, for the registers' sake)
+    int thread = threadIdx.x;
+    if constexpr (EVEN) asm volatile("" : "+v"(thread));
+    const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+    const int li = lane & 15, kg = lane >> 4;
+    const int slot = wave >> 1;
+    const bool keys = !(wave & 1), maker = wave < 4;
+    Part4 part;
+    if constexpr (EVEN) {
+      int parts;
+      int64_t at = same_in_all(state->at), end = same_in_all(state->end);
+      const bool some = next_part(late_args(), at, end, part, parts);
+      __syncthreads();                    // (the last part's reads of LDS too)
+      if (!some) break;
+      if (thread == 0) *state = EvenState{at, end, part};
+      if (part.va == 0) unused_splits(late_args(), part, parts);
     } else {
-      load_queries<E, W, NQ>(a, w, rows, kg, qf);
+      part = part_of_block(a);
     }
-    Sums4<W, NQ> sums(a);
-    float shift[NQ];
+    Walk4 w(g, part);
+    bool again = false;
+    if ((int64_t)w.rt0 * R < w.rows) {
+      w.tiles_of((int64_t)w.rt0 * R, min(w.rows, (int64_t)w.rt0 * R + R) - 1, a.group);
+      const unsigned d0 = 16 * NQ * wave;
+      const bool idle = w.r0 + d0 >= w.rows;
+      const int pairs = (w.tiles + 1) >> 1;
+      const Rows4<NQ> rows(g, w, d0, li);
+      // queries: as they are, or (float32) in bfloat16 terms
+      bf16x8 qf[NQ][KT][W];
+      if constexpr (KH) {
+        const _Float16 sign = a.scale < 0.0f ? (_Float16)-1.0f : (_Float16)1.0f;
 #pragma unroll
-    for (int q = 0; q < NQ; q++) shift[q] = 0.0f;
-
-    // A maker's tile on its way; where the halves of its next 32 tiles lie, one to a lane (a
-    // row of the pool, and whether the page is one in the highest bit).
-    unsigned char* raw = (unsigned char*)(flags + 16) + (wave & 3) * Raw4<W>::bytes;
-    const unsigned raw_at = __builtin_amdgcn_readfirstlane(
-        (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)raw);
-    const unsigned char *codes = keys ? a.kc : a.vc, *scales = keys ? a.ks : a.vs;
-    const int off = keys ? 2 : 1;         // pairs that its operands are made ahead
-    const int mine = maker ? (w.tiles - slot + 1) >> 1 : 0;      // its tiles
-    unsigned row_lo = 0, row_hi = 0;
-    int on = 0;                           // which halves of the tile on its way lie on pages
-    bool odd = false;                     // it has met what float16 does not hold
-    auto fetch = [&](int pair) __attribute__((always_inline)) {
-      if (pair >= mine) return;
-      if ((pair & 31) == 0) {
-        const int t = min(2 * (pair + (lane >> 1)) + slot, w.tiles - 1);
-        const int j = w.key_of(t) + 16 * (lane & 1);
-        const Attn4& c = late_args().a;
-        const int page = ((const int32_t*)w.table)[min(j, w.ghi - 1) >> c.shift];
-        const bool there = page >= 0 && page < c.n_pages;
-        const int64_t row = (((int64_t)(there ? page : 0) * c.heads + w.h) << c.shift) + (j & ((1 << c.shift) - 1));
-        row_lo = (unsigned)row;
-        row_hi = (unsigned)(row >> 32) | (there ? 0x80000000u : 0u);
-      }
-      const int at = 2 * (pair & 31);
-      const unsigned h0 = __builtin_amdgcn_readlane(row_hi, at), h1 = __builtin_amdgcn_readlane(row_hi, at + 1);
-      const unsigned l0 = __builtin_amdgcn_readlane(row_lo, at), l1 = __builtin_amdgcn_readlane(row_lo, at + 1);
-      on = (int)(h0 >> 31 | (h1 >> 31) << 1);
-      // (the reads of what lies there have ended: their values are used)
-      fetch_tile<W>((int64_t)(h0 & 0x7fffffffu) << 32 | l0, (int64_t)(h1 & 0x7fffffffu) << 32 | l1, codes, scales,
-                    raw_at, lane);
-    };
-    auto make = [&](int pair) __attribute__((always_inline)) {
-      if (!maker || pair >= pairs) return;
-      u32x4* to = lds + ((keys ? 0 : 4) + 2 * (pair & 1) + slot) * kHalf + lane;
-      const bool there = pair < mine;
-      wait_vmcnt<0>();
-      __asm__ volatile("" ::: "memory");
-      if (keys) {
-        if (lane == 0) flags[2 * (pair & 3) + slot] = there ? on : 0;
-        KeyTile<W> kt;
-        take_keys<W>(raw, li, kg, kt);
-#pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int q = 0; q < NQ; q++)
 #pragma unroll
           for (int n = 0; n < W; n++) {
-            if constexpr (KH) {
-              const unsigned s0 = kt.s[u][0], s1 = kt.s[u][Lane<W>::kblocks - 1];
-              const unsigned sc = f16_scale((W * kg + n) / 4 == W * kg / 4 ? s0 : s1, kt.w[u][n]);
-              odd |= there && !f16_holds(sc);
-              to[(u * W + n) * 64] = __builtin_bit_cast(u32x4, fp4_word_f16(kt.w[u][n], scale_of_byte(sc)));
-            } else {
-              to[(u * W + n) * 64] = __builtin_bit_cast(u32x4, key_operand<W>(kt, kg, u, n));
-            }
+            f16x8 v;
+            __builtin_memcpy(&v, (const _Float16*)a.q + (w.t0 + rows.tok[q]) * a.qt + rows.head[q] * a.qh +
+                                     8 * (W * kg + n), 16);
+            qf[q][0][n] = __builtin_bit_cast(bf16x8, v * sign);
           }
       } else {
-        ValueTile<W> vt;
-        take_values<W>(raw, li, kg, vt);
-        // (of a tile that is none: zeros, as of keys that no row sees)
-        clear_unseen<W>(w, vt, there && (on & 1), there && (on & 2), w.key_of(2 * pair + slot), kg);
-        if constexpr (VH) {
-          unsigned lo = 255, hi = 0;
+        load_queries<E, W, NQ>(a, w, rows, kg, qf);
+      }
+      Sums4<W, NQ> sums(a);
+      float shift[NQ];
 #pragma unroll
-          for (int e = 0; e < 8; e++)
+      for (int q = 0; q < NQ; q++) shift[q] = 0.0f;
+
+      // A maker's tile on its way; where the halves of its next 32 tiles lie, one to a lane (a
+      // row of the pool, and whether the page is one in the highest bit).
+      unsigned char* raw = (unsigned char*)(flags + 64) + (wave & 3) * Raw4<W>::bytes;
+      const unsigned raw_at = __builtin_amdgcn_readfirstlane(
+          (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)raw);
+      const unsigned char *codes = keys ? a.kc : a.vc, *scales = keys ? a.ks : a.vs;
+      const int off = keys ? 2 : 1;         // pairs that its operands are made ahead
+      const int mine = maker ? (w.tiles - slot + 1) >> 1 : 0;      // its tiles
+      unsigned row_lo = 0, row_hi = 0;
+      int on = 0;                           // which halves of the tile on its way lie on pages
+      bool odd = false;                     // it has met what float16 does not hold
+      auto fetch = [&](int pair) __attribute__((always_inline)) {
+        if (pair >= mine) return;
+        if ((pair & 31) == 0) {
+          const int t = min(2 * (pair + (lane >> 1)) + slot, w.tiles - 1);
+          const int j = w.key_of(t) + 16 * (lane & 1);
+          const Attn4& c = late_args().a;
+          const int page = ((const int32_t*)w.table)[min(j, w.ghi - 1) >> c.shift];
+          const bool there = page >= 0 && page < c.n_pages;
+          const int64_t row = (((int64_t)(there ? page : 0) * c.heads + w.h) << c.shift) + (j & ((1 << c.shift) - 1));
+          row_lo = (unsigned)row;
+          row_hi = (unsigned)(row >> 32) | (there ? 0x80000000u : 0u);
+        }
+        const int at = 2 * (pair & 31);
+        const unsigned h0 = __builtin_amdgcn_readlane(row_hi, at), h1 = __builtin_amdgcn_readlane(row_hi, at + 1);
+        const unsigned l0 = __builtin_amdgcn_readlane(row_lo, at), l1 = __builtin_amdgcn_readlane(row_lo, at + 1);
+        on = (int)(h0 >> 31 | (h1 >> 31) << 1);
+        // (the reads of what lies there have ended: their values are used)
+        fetch_tile<W>((int64_t)(h0 & 0x7fffffffu) << 32 | l0, (int64_t)(h1 & 0x7fffffffu) << 32 | l1, codes, scales,
+                      raw_at, lane);
+      };
+      auto make = [&](int pair) __attribute__((always_inline)) {
+        if (!maker || pair >= pairs) return;
+        // (its addresses are found anew each time: they would take registers from the products)
+        int lane = threadIdx.x & 63;
+        if constexpr (EVEN) asm volatile("" : "+v"(lane));
+        const int li = lane & 15, kg = lane >> 4;
+        u32x4* to = lds + ((keys ? 0 : 4) + 2 * (pair & 1) + slot) * kHalf + lane;
+        const bool there = pair < mine;
+        wait_vmcnt<0>();
+        __asm__ volatile("" ::: "memory");
+        if (keys) {
+          if (lane == 0) flags[2 * (pair & 3) + slot] = there ? on : 0;
+          KeyTile<W> kt;
+          take_keys<W>(raw, li, kg, kt);
 #pragma unroll
-            for (int i = 0; i < Lane<W>::vblocks; i++) {
-              lo = min(lo, vt.s[e][i]);
-              hi = max(hi, vt.s[e][i]);
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int n = 0; n < W; n++) {
+              if constexpr (KH) {
+                const unsigned s0 = kt.s[u][0], s1 = kt.s[u][Lane<W>::kblocks - 1];
+                const unsigned sc = f16_scale((W * kg + n) / 4 == W * kg / 4 ? s0 : s1, kt.w[u][n]);
+                odd |= there && !f16_holds(sc);
+                to[(u * W + n) * 64] = __builtin_bit_cast(u32x4, fp4_word_f16(kt.w[u][n], scale_of_byte(sc)));
+              } else {
+                to[(u * W + n) * 64] = __builtin_bit_cast(u32x4, key_operand<W>(kt, kg, u, n));
+              }
             }
-          if (__any(!f16_holds(lo) || !f16_holds(hi))) {
+        } else {
+          ValueTile<W> vt;
+          take_values<W>(raw, li, kg, vt);
+          // (of a tile that is none: zeros, as of keys that no row sees)
+          clear_unseen<W>(w, vt, there && (on & 1), there && (on & 2), w.key_of(2 * pair + slot), kg);
+          if constexpr (VH) {
+            unsigned lo = 255, hi = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++)
 #pragma unroll
               for (int i = 0; i < Lane<W>::vblocks; i++) {
-                unsigned codes = 0;
-#pragma unroll
-                for (int x = 0; x < Lane<W>::vwords; x++) codes |= vt.w[e][x];
-                vt.s[e][i] = f16_scale(vt.s[e][i], codes);
-                odd |= !f16_holds(vt.s[e][i]);
+                lo = min(lo, vt.s[e][i]);
+                hi = max(hi, vt.s[e][i]);
               }
+            if (__any(!f16_holds(lo) || !f16_holds(hi))) {
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+#pragma unroll
+                for (int i = 0; i < Lane<W>::vblocks; i++) {
+                  unsigned codes = 0;
+#pragma unroll
+                  for (int x = 0; x < Lane<W>::vwords; x++) codes |= vt.w[e][x];
+                  vt.s[e][i] = f16_scale(vt.s[e][i], codes);
+                  odd |= !f16_holds(vt.s[e][i]);
+                }
+            }
           }
+          Place<W> place(li, kg);
+          place.shift = 0;
+          value_operands<W, VH>(vt, place, li, [&](int x, u32x4 v) __attribute__((always_inline)) { to[x * 64] = v; });
         }
-        Place<W> place(li, kg);
-        place.shift = 0;
-        value_operands<W, VH>(vt, place, li, [&](int x, u32x4 v) __attribute__((always_inline)) { to[x * 64] = v; });
-      }
-      __asm__ volatile("" ::: "memory");
-    };
+        __asm__ volatile("" ::: "memory");
+      };
 
-    f32x4 s[2][2][NQ];                     // scores of a pair
-    float mc[NQ];
-    u32x4 kf[2 * W], vf[2][W];
-    auto read_keys = [&](int buffer, int i) __attribute__((always_inline)) {
-      const u32x4* from = lds + (2 * buffer + i) * kHalf + lane;
+      f32x4 s[2][2][NQ];                     // scores of a pair
+      float mc[NQ];
+      u32x4 kf[2 * W], vf[2][W];
+      auto read_keys = [&](int buffer, int i) __attribute__((always_inline)) {
+        const u32x4* from = lds + (2 * buffer + i) * kHalf + lane;
 #pragma unroll
-      for (int x = 0; x < 2 * W; x++) kf[x] = from[x * 64];
-    };
-    auto read_values = [&](int buffer, int i, int half) __attribute__((always_inline)) {
-      const u32x4* from = lds + (4 + 2 * buffer + i) * kHalf + half * W * 64 + lane;
+        for (int x = 0; x < 2 * W; x++) kf[x] = from[x * 64];
+      };
+      auto read_values = [&](int buffer, int i, int half) __attribute__((always_inline)) {
+        const u32x4* from = lds + (4 + 2 * buffer + i) * kHalf + half * W * 64 + lane;
 #pragma unroll
-      for (int x = 0; x < W; x++) vf[half][x] = from[x * 64];
-    };
-    auto scores = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int q = 0; q < NQ; q++) s[i][u][q] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int n = 0; n < W; n++)
+        for (int x = 0; x < W; x++) vf[half][x] = from[x * 64];
+      };
+      auto scores = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-          for (int q = 0; q < NQ; q++) {
-            const u32x4 k = kf[u * W + n];
-            if constexpr (KH) {
-              s[i][u][q] = mfma16h(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, qf[q][0][n]), s[i][u][q]);
-            } else {
+          for (int q = 0; q < NQ; q++) s[i][u][q] = f32x4{0, 0, 0, 0};
 #pragma unroll
-              for (int t = KT - 1; t >= 0; t--)
-                s[i][u][q] = mfma16(__builtin_bit_cast(bf16x8, k), qf[q][t][n], s[i][u][q]);
+        for (int n = 0; n < W; n++)
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int q = 0; q < NQ; q++) {
+              const u32x4 k = kf[u * W + n];
+              if constexpr (KH) {
+                s[i][u][q] = mfma16h(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, qf[q][0][n]), s[i][u][q]);
+              } else {
+#pragma unroll
+                for (int t = KT - 1; t >= 0; t--)
+                  s[i][u][q] = mfma16(__builtin_bit_cast(bf16x8, k), qf[q][t][n], s[i][u][q]);
+              }
             }
-          }
-    };
-    auto terms = [&](int i, bf16x8 (&pf)[NQ][PT]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int q = 0; q < NQ; q++) {
-        float p[8], sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          p[e] = exp2_(__builtin_fmaf(s[i][e / 4][q][e % 4], sums.c, -mc[q]));
-          sum = e ? sum + p[e] : p[e];
-        }
-        sums.l[q] += sum;
-        if constexpr (VH) {
-          f16x8 f;
-#pragma unroll
-          for (int e = 0; e < 8; e++) f[e] = (_Float16)p[e];
-          pf[q][0] = __builtin_bit_cast(bf16x8, f);
-          if constexpr (PT > 1) {
-            f16x8 f1;
-#pragma unroll
-            for (int e = 0; e < 8; e++) f1[e] = (_Float16)(p[e] - (float)f[e]);
-            pf[q][1] = __builtin_bit_cast(bf16x8, f1);
-          }
-        } else {
-          split8<PT, false>(p, pf[q]);
-        }
-      }
-    };
-    auto add_values = [&](const bf16x8 (&pf)[NQ][PT], int half) __attribute__((always_inline)) {
-#pragma unroll
-      for (int x = 0; x < W; x++)
-#pragma unroll
-        for (int q = 0; q < NQ; q++)
-#pragma unroll
-          for (int t = PT - 1; t >= 0; t--) {
-            f32x4& o = sums.o[q][half * W + x];
-            if constexpr (VH)
-              o = mfma16h(__builtin_bit_cast(f16x8, vf[half][x]), __builtin_bit_cast(f16x8, pf[q][t]), o);
-            else
-              o = mfma16(__builtin_bit_cast(bf16x8, vf[half][x]), pf[q][t], o);
-          }
-    };
-
-    // what the first round needs, and the loads of the next
-    fetch(0);
-    make(0);
-    if (keys) {
-      fetch(1);
-      make(1);
-    }
-    fetch(off);
-    // pairs of tiles that need no masks (where they lie on pages): behind the first tokens
-    const int clear0 = w.n1 + ((max(rows.all_lo - w.b0, 0) + 31) >> 5), clear1 = w.n1 + ((rows.all_hi - w.b0) >> 5);
-    __syncthreads();
-    if (!idle) {
-      read_keys(0, 0);
-      scores(0);
-      read_keys(0, 1);
-      scores(1);
-    }
-    __syncthreads();
-    for (int pair = 0; pair < pairs; pair++) {
-      const int on0 = flags[2 * (pair & 3)], on1 = flags[2 * (pair & 3) + 1];
-      make(pair + off);
-      fetch(pair + off + 1);
-      if (!idle) {
-        const int buffer = pair & 1;
-        // masks and maxima of the pair's scores
-        const int there0 = __builtin_amdgcn_readfirstlane(on0), there1 = __builtin_amdgcn_readfirstlane(on1);
-        if (2 * pair < clear0 || 2 * pair + 2 > clear1 || (there0 & there1) != 3) {
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const int there = i ? there1 : there0;
-            rows.mask(late_args(), w, w.key_of(2 * pair + i), kg, there & 1, there & 2, shift, s[i]);
-          }
-        }
-        bool grows = false;
-        float mx[NQ];
+      };
+      auto terms = [&](int i, bf16x8 (&pf)[NQ][PT]) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
-          mx[q] = s[0][0][q][0];
+          float p[8], sum = 0.0f;
 #pragma unroll
-          for (int e = 1; e < 16; e++) mx[q] = fmaxf(mx[q], s[e / 8][e / 4 % 2][q][e % 4]);
-          grows |= mx[q] > sums.m[q];
+          for (int e = 0; e < 8; e++) {
+            p[e] = exp2_(__builtin_fmaf(s[i][e / 4][q][e % 4], sums.c, -mc[q]));
+            sum = e ? sum + p[e] : p[e];
+          }
+          sums.l[q] += sum;
+          if constexpr (VH) {
+            f16x8 f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = (_Float16)p[e];
+            pf[q][0] = __builtin_bit_cast(bf16x8, f);
+            if constexpr (PT > 1) {
+              f16x8 f1;
+#pragma unroll
+              for (int e = 0; e < 8; e++) f1[e] = (_Float16)(p[e] - (float)f[e]);
+              pf[q][1] = __builtin_bit_cast(bf16x8, f1);
+            }
+          } else {
+            split8<PT, false>(p, pf[q]);
+          }
         }
-        // (all lanes or none; said as each lane's own choice, for which the compiler scales
-        // the sums where they are: else it copies all of them every round, 5% of the time)
-        const bool some = __any(grows);
-        if (grows | some) {
+      };
+      auto add_values = [&](const bf16x8 (&pf)[NQ][PT], int half) __attribute__((always_inline)) {
 #pragma unroll
-          for (int q = 0; q < NQ; q++) sums.raise_to(q, column_max(mx[q]));
-        }
+        for (int x = 0; x < W; x++)
 #pragma unroll
-        for (int q = 0; q < NQ; q++) mc[q] = sums.offset(q) - (VH ? kHigh : 0.0f);
-        // The pair's terms and their products with the values; between them the next
-        // pair's scores (the last round's are of nothing and not used).  Operands are
-        // read a step ahead of their products.
-        bf16x8 p0[NQ][PT], p1[NQ][PT];
-        read_keys(buffer ^ 1, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        terms(0, p0);
-        read_values(buffer, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int t = PT - 1; t >= 0; t--) {
+              f32x4& o = sums.o[q][half * W + x];
+              if constexpr (VH)
+                o = mfma16h(__builtin_bit_cast(f16x8, vf[half][x]), __builtin_bit_cast(f16x8, pf[q][t]), o);
+              else
+                o = mfma16(__builtin_bit_cast(bf16x8, vf[half][x]), pf[q][t], o);
+            }
+      };
+
+      // what the first round needs, and the loads of the next
+      fetch(0);
+      make(0);
+      if (keys) {
+        fetch(1);
+        make(1);
+      }
+      fetch(off);
+      // pairs of tiles that need no masks (where they lie on pages): behind the first tokens
+      const int clear0 = w.n1 + ((max(rows.all_lo - w.b0, 0) + 31) >> 5), clear1 = w.n1 + ((rows.all_hi - w.b0) >> 5);
+      __syncthreads();
+      if (!idle) {
+        read_keys(0, 0);
         scores(0);
-        read_values(buffer, 0, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        add_values(p0, 0);
-        add_values(p0, 1);
-        read_keys(buffer ^ 1, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        terms(1, p1);
-        read_values(buffer, 1, 0);
-        __builtin_amdgcn_sched_barrier(0);
+        read_keys(0, 1);
         scores(1);
-        read_values(buffer, 1, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        add_values(p1, 0);
-        add_values(p1, 1);
       }
       __syncthreads();
-    }
-    again = sums.unsure();
-    if constexpr (VH) {
-      if (lane == 0) flags[wave] = 0;
-      if (odd) flags[wave] = 1;
-      __syncthreads();
-      for (int i = 0; i < waves; i++) again |= flags[i] != 0;
-      again = __any(again);
-    }
-    if (!idle && !again) {
+      for (int pair = 0; pair < pairs; pair++) {
+        const int on0 = flags[2 * (pair & 3)], on1 = flags[2 * (pair & 3) + 1];
+        make(pair + off);
+        fetch(pair + off + 1);
+        if (!idle) {
+          const int buffer = pair & 1;
+          // masks and maxima of the pair's scores
+          const int there0 = __builtin_amdgcn_readfirstlane(on0), there1 = __builtin_amdgcn_readfirstlane(on1);
+          if (2 * pair < clear0 || 2 * pair + 2 > clear1 || (there0 & there1) != 3) {
 #pragma unroll
-      for (int q = 0; q < NQ; q++) {
-        sums.l[q] = column_sum(sums.l[q]);
-        if constexpr (VH) {
-          sums.l[q] *= 0x1p-14f;
+            for (int i = 0; i < 2; i++) {
+              const int there = i ? there1 : there0;
+              rows.mask(late_args(), w, w.key_of(2 * pair + i), kg, there & 1, there & 2, shift, s[i]);
+            }
+          }
+          bool grows = false;
+          float mx[NQ];
 #pragma unroll
-          for (int x = 0; x < 2 * W; x++)
+          for (int q = 0; q < NQ; q++) {
+            mx[q] = s[0][0][q][0];
 #pragma unroll
-            for (int r = 0; r < 4; r++) sums.o[q][x][r] *= 0x1p-14f;
+            for (int e = 1; e < 16; e++) mx[q] = fmaxf(mx[q], s[e / 8][e / 4 % 2][q][e % 4]);
+            grows |= mx[q] > sums.m[q];
+          }
+          // (all lanes or none; said as each lane's own choice, for which the compiler scales
+          // the sums where they are: else it copies all of them every round, 5% of the time)
+          const bool some = __any(grows);
+          if (grows | some) {
+#pragma unroll
+            for (int q = 0; q < NQ; q++) sums.raise_to(q, column_max(mx[q]));
+          }
+#pragma unroll
+          for (int q = 0; q < NQ; q++) mc[q] = sums.offset(q) - (VH ? kHigh : 0.0f);
+          // The pair's terms and their products with the values; between them the next
+          // pair's scores (the last round's are of nothing and not used).  Operands are
+          // read a step ahead of their products.
+          bf16x8 p0[NQ][PT], p1[NQ][PT];
+          read_keys(buffer ^ 1, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          terms(0, p0);
+          read_values(buffer, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          scores(0);
+          read_values(buffer, 0, 1);
+          __builtin_amdgcn_sched_barrier(0);
+          add_values(p0, 0);
+          add_values(p0, 1);
+          read_keys(buffer ^ 1, 1);
+          __builtin_amdgcn_sched_barrier(0);
+          terms(1, p1);
+          read_values(buffer, 1, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          scores(1);
+          read_values(buffer, 1, 1);
+          __builtin_amdgcn_sched_barrier(0);
+          add_values(p1, 0);
+          add_values(p1, 1);
         }
+        __syncthreads();
       }
-      // (found anew: out of the compiler's sight, which would keep them through the walk)
-      int lanes = li;
-      asm volatile("" : "+v"(lanes));
-      const Rows4<NQ> at(late_args(), w, d0, lanes);
-      store_rows<E, W, NQ, 4>(late_args().a, w, at, kg, 0, sums.m, sums.l, sums.o);
+      again = sums.unsure();
+      if constexpr (VH) {
+        if (lane == 0) flags[wave] = 0;
+        if (odd) flags[wave] = 1;
+        __syncthreads();
+        for (int i = 0; i < waves; i++) again |= flags[i] != 0;
+        again = __any(again);
+      }
+      if (!idle && !again) {
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+          sums.l[q] = column_sum(sums.l[q]);
+          if constexpr (VH) {
+            sums.l[q] *= 0x1p-14f;
+#pragma unroll
+            for (int x = 0; x < 2 * W; x++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) sums.o[q][x][r] *= 0x1p-14f;
+          }
+        }
+        // (found anew: out of the compiler's sight, which would keep them through the walk)
+        int lanes = li;
+        asm volatile("" : "+v"(lanes));
+        const Rows4<NQ> at(late_args(), w, d0, lanes);
+        store_rows<E, W, NQ, 4>(late_args().a, w, at, kg, 0, sums.m, sums.l, sums.o);
+      }
     }
+    // rows to be walked again, and those of a sequence with more than max_new bounds
+    const Mask4& late = late_args();
+    for (int64_t tile = (int64_t)w.rt0 + (again ? 0 : late.a.row_tiles); tile * R < w.rows; tile += late.a.row_tiles) {
+      const Part4 p = EVEN ? state->part : part_of_block(late.a);
+      slow_rows<E, W, NQ>(&late, p.b, p.h, p.rt0, p.split, p.va, p.vb, tile * R, R);
+    }
+    if constexpr (!EVEN) break;
   }
-  // rows to be walked again, and those of a sequence with more than max_new bounds
-  const Mask4& late = late_args();
-  for (int64_t tile = (int64_t)w.rt0 + (again ? 0 : late.a.row_tiles); tile * R < w.rows; tile += late.a.row_tiles)
-    slow_rows<E, W, NQ>(&late, tile * R, R);
 }
 
 // How a call is run: waves of a workgroup that share tiles (0: few rows), column tiles
 // a wave.
 struct Mask4Plan {
-  int nq, waves, few;             // (few: waves that share few rows)
+  int nq, waves, few, even;       // (few: waves that share few rows; even: even shares)
   int row_tiles, splits;
   int64_t chunk;
   size_t workspace;
@@ -1121,18 +1255,21 @@ static int launch_mask4_few(const Mask4& g, int few, hipStream_t s) {
   return launch_check("mask4_few_kernel");
 }
 
-template <typename E, int W, int NQ>
+template <typename E, int W, int NQ, bool EVEN>
 static int launch_mask4_shared(const Mask4& g, int waves, hipStream_t s) {
-  const size_t lds = (size_t)16 * W * 1024 + 64 + 4 * Raw4<W>::bytes;
-  if (lds > 65536) QPH_TRY(allow_full_lds((const void*)mask4_shared_kernel<E, W, NQ>));
-  const int64_t blocks = (int64_t)g.a.row_tiles * g.a.splits * g.a.heads * g.a.batch;
-  hipLaunchKernelGGL((mask4_shared_kernel<E, W, NQ>), dim3((unsigned)blocks), dim3(64 * waves), lds, s, g);
+  const size_t lds = (size_t)16 * W * 1024 + 256 + 4 * Raw4<W>::bytes;
+  if (lds > 65536) QPH_TRY(allow_full_lds((const void*)mask4_shared_kernel<E, W, NQ, EVEN>));
+  const int64_t blocks = EVEN ? (waves > 4 ? 256 : 512)
+                                : (int64_t)g.a.row_tiles * g.a.splits * g.a.heads * g.a.batch;
+  hipLaunchKernelGGL((mask4_shared_kernel<E, W, NQ, EVEN>), dim3((unsigned)blocks), dim3(64 * waves), lds, s, g);
   return launch_check("mask4_shared_kernel");
 }
 
 template <typename E, int W>
 static int launch_mask4_w(const Mask4& g, const Mask4Plan& p, hipStream_t s) {
-  if (p.waves) return launch_mask4_shared<E, W, mask4_nq(E::terms, W)>(g, p.waves, s);
+  constexpr int NQ = mask4_nq(E::terms, W);
+  if (p.even) return launch_mask4_shared<E, W, NQ, true>(g, p.waves, s);
+  if (p.waves) return launch_mask4_shared<E, W, NQ, false>(g, p.waves, s);
   if constexpr (mask4_nq(E::terms, W) == 2) {
     if (p.nq == 2) return launch_mask4_few<E, W, 2>(g, p.few, s);
   }

@@ -115,6 +115,17 @@ static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_a
   // are kept: eight waves a workgroup leave some CUs two (40 sequences: 58 us, 47 with splits).
   r.few = !r.waves && r.nq == 1 && n == 3 && blocks <= 256 ? mask4_few_waves<1>(terms, w) : 4;
   if (r.few > 4) n = 1;
+  // Several sequences of one row tile each: even shares of all their keys, which the
+  // workgroups find from the lengths (each lane one sequence's), in place of splits of as many
+  // keys, of which the chip had to wait for the last full ones (trees of 32 tokens, ragged
+  // sequences, 8 heads: 32 of up to 8192 keys 135 us, 156 with equal splits; 6 of up to 32000
+  // 124, 149; equal lengths: the same).  A sequence has at most twice the parts that all
+  // have on average, and two that begin or end inside a share.
+  if (n > 1 && r.waves && r.row_tiles == 1 && p->batch > 1 && p->batch <= 64) {
+    r.even = 1;
+    r.splits = (int)std::min<int64_t>(2 * (r.waves > 4 ? 256 : 512) / blocks + 2, 64);
+    n = 1;
+  }
   if (n > 1) {
     r.chunk = ((keys + n - 1) / n + 127) / 128 * 128;
     n = (keys + r.chunk - 1) / r.chunk;

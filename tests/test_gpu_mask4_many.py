@@ -272,3 +272,111 @@ def test_captured(gpu, length):
             y2, s2 = ops.attention_tree4(q, c, table, lens, 0.1, t, lse=True)
             assert (host(y) == host(y2)).all() and (host(s) == host(s2)).all()
             assert np.isfinite(host(y)).all() and not (host(s) == -math.inf).any()
+
+
+# ------------------------------------- several sequences of a row tile, even shares of their keys
+
+EVEN = 1 << 20            # a bound for which keys are split however short the sequences are
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dh", HEAD_DIMS)
+@pytest.mark.parametrize("heads,group,news,context,window,sinks,tree", [
+    (2, 4, [31, 0, 1, 17, 9], [4000, 50, 0, 700, 2100], 0, 0, True),
+    (1, 8, [16, 15, 2], [33, 2900, 0], 0, 0, True),
+    (1, 3, [20, 33, 7, 1, 40], [64, 1000, 0, 31, 1900], 500, 70, True),
+    (3, 1, [60, 90], [1500, 1700], 1030, 5, False),
+    (1, 2, [50, 13, 64], [900, 0, 2500], 0, 0, False)])
+def test_even_shares(gpu, dtype, dh, heads, group, news, context, window, sinks, tree):
+    print("even", dtype, dh, heads, group, news, context, window, sinks, tree, flush=True)
+    rng = np.random.default_rng(dh + sum(news) + group)
+    lens = [a + b for a, b in zip(context, news)]
+    c, table = setup(gpu, rng, lens, heads, dh, 32)
+    trees = [paths(drafted(rng, n, 5)) for n in news] if tree else None
+    q = queries(gpu, rng, sum(news), heads * group, dh, dtype)
+    got = [check(gpu, c, q, table, lens, news, window, sinks, trees, rows=some(news, 5), max_len=bound,
+                 causal=group != 2) for bound in (EVEN, max(lens), EVEN)]
+    assert (got[0][0] == got[2][0]).all() and (got[0][1] == got[2][1]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch", [2, 30, 64, 65])
+def test_even_shares_of_short_sequences(gpu, dtype, batch):
+    """Many parts to a workgroup; one long sequence among short ones; as many sequences as
+    a wave has lanes, and one more."""
+    rng = np.random.default_rng(batch)
+    lens = [int(x) for x in rng.integers(0, 200, batch)]
+    lens[batch // 2] = 3000
+    news = [int(x) for x in rng.integers(0, 9, batch)]
+    news[-1], news[batch // 2] = 20, 20
+    c, table = setup(gpu, rng, lens, 1, 64, 16)
+    q = queries(gpu, rng, sum(news), 8, 64, dtype)
+    trees = [paths(drafted(rng, n, 5)) for n in news]
+    print("short", dtype, batch, flush=True)
+    check(gpu, c, q, table, lens, news, trees=trees, rows=some(news, 2), max_len=EVEN)
+    check(gpu, c, q, table, lens, news, 50, 33, rows=some(news, 2), max_len=EVEN)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dh", [64, 192])
+def test_even_shares_walked_again(gpu, dtype, dh):
+    """Values that float16 does not hold, NaN, and scores far from zero in some parts of a
+    sequence; lengths past the table and below zero; pages outside the pool."""
+    rng = np.random.default_rng(dh)
+    lens, news, group = [1900, 700, 1 << 20, -5, 64], [16, 9, 12, 3, 16], 8
+    c, table = setup(gpu, rng, [1900, 700, 90, 0, 64], 1, dh, 32)
+    wide = max(len(t) for t in table)
+    table = [t + [-1] * (wide - len(t)) for t in table]
+    table[1][3] = c.pages
+    for b, j, scale in ((0, 30, 145), (0, 1700, 100), (1, 400, 142), (4, 5, 103)):
+        c.v_scales[table[b][j // 32], :, j % 32] = scale
+    for b, j, scale in ((0, 900, 142), (1, 5, 255), (4, 50, 150)):
+        c.k_scales[table[b][j // 32], :, j % 32] = scale
+    c.v_scales[table[0][1890 // 32], :, 1890 % 32] = 255         # a drafted token
+    q = queries(gpu, rng, sum(news), group, dh, dtype)
+    trees = [paths(drafted(rng, n, 4)) for n in news]
+    print("again", dtype, dh, flush=True)
+    check(gpu, c, q, table, lens, news, trees=trees, max_len=EVEN)
+    check(gpu, c, q, table, lens, news, 700, 31, max_len=EVEN)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_even_shares_past_the_bound(gpu, dtype):
+    """Sequences with more new tokens than max_new, their further rows in the same parts;
+    captured and replayed with other lengths."""
+    from qppocr_amd import ops
+    rng = np.random.default_rng(4)
+    news, dh, group = [130, 20], 64, 8
+    c = make_cache(gpu, rng, 80, 32, 1, dh)
+    table = gpu.from_numpy(rng.permutation(80).reshape(2, 40).astype(np.int32)).cuda()
+    q = queries(gpu, rng, 150, group, dh, dtype)
+    trees = [paths(drafted(rng, n, 4)) for n in news]
+    bits = np.zeros((150, 3), dtype=np.int64)
+    bits[:130], bits[130:] = words_of(trees[0], 3), words_of(trees[1], 3)
+    words = gpu.from_numpy(bits).cuda()
+    st = gpu.tensor([0, 130, 150], dtype=gpu.int32, device="cuda")
+    ln = gpu.tensor([1200, 900], dtype=gpu.int32, device="cuda")
+
+    def call(bound, most=EVEN):
+        return ops.attention_tree4(q, c, table, ln, 0.125, words, starts=st, max_new=bound, max_len=most, lse=True)
+    call(20)
+    g = gpu.cuda.CUDAGraph()
+    with gpu.cuda.graph(g):
+        y, s = call(20)
+    terms = {"float32": 3, "float16": 2, "bfloat16": 1}[dtype]
+    k, v = numbers(c)
+    for lens in ([1200, 900], [131, 1280], [1280, 20]):
+        ln.copy_(gpu.tensor(lens, dtype=gpu.int32))
+        gpu.cuda.synchronize()
+        g.replay()
+        gpu.cuda.synchronize()
+        y2, s2 = call(20)
+        assert (host(y) == host(y2)).all() and (host(s) == host(s2)).all()
+        for b, i in some(news, 8):
+            pos = np.arange(lens[b])
+            pg = host(table)[b].astype(np.int64)[pos // 32]
+            see = visible(lens[b], news[b], i, True, 0, 0, trees[b])
+            want, tol, (lse, ltol) = attend(host(q)[130 * b + i], k[pg[see], pos[see] % 32],
+                                            v[pg[see], pos[see] % 32], 0.125, terms, group)
+            close(host(y)[130 * b + i], want, tol + half_step(gpu, q.dtype, want) * 1.001, f"row {b} {i}")
+            close(host(s)[130 * b + i], lse, ltol, f"lse {b} {i}")
