@@ -8,10 +8,17 @@
 // qph_attn4.hip.  Two forms:
 //
 // Few rows of a sequence and head: the waves of a workgroup share 16 NQ rows and take
-// the tiles of 32 keys in turn, codes to registers to operands.
+// the tiles of 32 keys in turn, codes to registers to operands.  Bound by the codes' way
+// from memory: one token of 32 sequences with 4100 of their keys (8 heads of 128) 143 MB in
+// 36.7 us, 3.9 TB/s where a large copy runs at 4.6.
 //
 // Many (mask4_shared_kernel): each wave has 16 NQ rows of its own, so every tile is
-// needed by all waves, and its codes are turned into operands once, by way of LDS.
+// needed by all waves, and its codes are turned into operands once, by way of LDS.  Bound
+// by what the SIMDs issue beside their products and by LDS: 1024 new tokens of two
+// sequences with windows of 2000 (bfloat16, 32 heads of 128 over 8) 68 GF in 89 us, 770
+// TFLOP/s where a large library product runs at 1134; a round of 64 keys takes about 5000
+// cycles, of which the matrix unit has work for 2050, the vector instructions of two waves
+// fill 2600 and the operands' reads of LDS 2300.
 //
 // Keys are walked as two runs of tiles: the first tokens, and what lies in the
 // window of any row of the workgroup, up to the last key.  A tile inside every row's
@@ -736,8 +743,8 @@ __device__ __forceinline__ f32x4 mfma16h(f16x8 a, f16x8 b, f32x4 c) {
 
 // The products' types.  With float16 queries the scores are float16 products, and
 // with queries of either two-byte type the second products are: one term of a
-// bfloat16 row's probabilities (11 bits: the row is rounded to 8), two of a float16
-// row's.  Probabilities stand 2^14 higher there, so that float16 holds them down to
+// bfloat16 row's probabilities (11 bits: the row is rounded to 8; with two, chunks with
+// sinks 119 us for 95 and ragged trees 232 for 185), two of a float16 row's.  Probabilities stand 2^14 higher there, so that float16 holds them down to
 // 2^-28 in full and to 2^-38 at all.  Keys or values past what float16 holds send the
 // workgroup's rows through the second walk, which is in bfloat16 terms, as all of
 // float32 is: a choice between two products in every tile has the sums held twice.
@@ -887,7 +894,8 @@ __device__ __noinline__ void slow_rows(const Mask4* g, int b, int h, int rt0, in
 // of the next pair, whose scores then lie in the registers of the pair before (so the
 // matrix unit has work while the exponentials of the other tile are taken); keys of the
 // pair after that and values of the next are turned; and the codes of one pair more
-// are on their way.
+// are on their way.  (Two halves of the waves in opposite phases, one multiplying while the
+// other turns codes and takes exponentials, were slower: 119 us for 96.)
 template <typename E, int W, int NQ, bool EVEN>
 __global__ __launch_bounds__(64 * mask4_waves(E::terms, W), mask4_waves(E::terms, W) / 4) void
 mask4_shared_kernel(Mask4 g) {

@@ -169,7 +169,9 @@ __device__ __forceinline__ unsigned ring_place(int64_t at, unsigned n) {
 // sums itself (in LDS): a second launch, or a wait for another workgroup, costs
 // more than the few thousand additions.  A row's page comes from the table where
 // its sequence had the page before, and else from the ring, not from the entry
-// that another thread writes now.
+// that another thread writes now.  Bound by trips to memory one after the other
+// (lengths, sums, a page, its entry, a parent): 48 trees of up to 32 tokens 8.4
+// us, 384 prompts of some 940000 tokens in all (11 MB) 12.8.
 template <bool FEW>
 __global__ __launch_bounds__(256) void extend4_kernel(Extend4 a) {
   __shared__ int lds[FEW ? 3 * (kExtendFew + 1) : 1];
@@ -354,7 +356,9 @@ __device__ __forceinline__ void cos_sin(u64 phase, float* c, float* s) {
 
 // A thread has V pairs of a token, computes their cosines and sines once and turns
 // them in `each` heads.  The position times the turns a position, in 2^-64ths, is
-// exact modulo a turn in 64 bits, however far the position.
+// exact modulo a turn in 64 bits, however far the position.  Bound by memory: 20011
+// tokens of 40 heads of 128 in bfloat16 (410 MB) 97 us, 4.2 TB/s where a large copy
+// runs at 4.6; 32 tokens of them 5.0 us, a launch and two trips to memory.
 template <typename E, int V, bool NB>
 __global__ __launch_bounds__(256) void rotary_kernel(Rotary a) {
   typedef typename E::type T;
@@ -463,7 +467,8 @@ __device__ __forceinline__ int64_t move_block(const Move4& a, int64_t slot, unsi
 }
 
 // A few tokens: a workgroup has all of them for its head's keys or values, reads
-// all, then writes all, so that a place may be left and taken in one call.
+// all, then writes all, so that a place may be left and taken in one call.  (190
+// tokens of 8 heads of 128: 2.7 us, a launch and three trips to memory.)
 template <int U>
 __global__ __launch_bounds__(1024) void move4_few_kernel(Move4 a) {
   const unsigned h = blockIdx.x >> 1, second = blockIdx.x & 1;
@@ -495,6 +500,7 @@ __global__ __launch_bounds__(1024) void move4_few_kernel(Move4 a) {
 }
 
 // Many tokens: out of the cache into the workspace, and in another launch back.
+// (16001 tokens of 8 heads of 128, 35 MB read and written twice: 10.0 and 8.9 us.)
 template <bool BACK>
 __global__ __launch_bounds__(256) void move4_many_kernel(Move4 a) {
   const unsigned units = 2 * a.heads * a.blocks;

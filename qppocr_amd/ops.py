@@ -4,13 +4,14 @@ sgemm / sgemm_res, matmul, softmax_last_dim, gelu_inplace, hardsigmoid,
 sigmoid_tensor, relu_inplace, reduce_mean (last axis), resize_nearest, and the
 CTC argmax of qppocr-core/src/pipeline/rec.rs; and the 4-bit operators of a
 token-by-token decoder (quantize4, linear4, cache4_write, cache4_read,
-attention_cache4), which the reference lacks.
+attention_cache4; of its steps cache4_extend, rotary, attention_tree4,
+cache4_move), which the reference lacks.
 
 Tensors are torch tensors on a ROCm device (torch is only the device-memory
 plumbing here); every call goes through the C ABI of libqppocr_hip.so.  Calls
 are synchronous with respect to torch's current stream: the stream is drained
 before the library's own stream runs the kernel, and the library stream is
-drained before returning.  The 4-bit operators do not wait: they are enqueued on
+drained before returning.  A decoder's operators do not wait: they are enqueued on
 torch's current stream of the tensors' device, in its order, and may be captured
 into a graph; they compute no gradients and refuse tensors that require one.
 Errors raise QphError (no silent fallback).

@@ -380,3 +380,23 @@ def test_even_shares_past_the_bound(gpu, dtype):
                                             v[pg[see], pos[see] % 32], 0.125, terms, group)
             close(host(y)[130 * b + i], want, tol + half_step(gpu, q.dtype, want) * 1.001, f"row {b} {i}")
             close(host(s)[130 * b + i], lse, ltol, f"lse {b} {i}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("part", ["v", "k"])
+def test_numbers_below_the_smallest_normal_float16(gpu, dtype, part):
+    """All values, then all keys, so small that float16 holds them below its normal
+    numbers: nothing of them is lost."""
+    rng = np.random.default_rng(44)
+    lens, news, group, dh = [300], [70], 4, 64
+    c, table = setup(gpu, rng, lens, 1, dh, 32)
+    s = getattr(c, part + "_scales")
+    s.copy_(gpu.from_numpy(rng.integers(104, 109, s.shape).astype(np.uint8)))
+    q = queries(gpu, rng, 70, group, dh, dtype)
+    trees = [paths(drafted(rng, 70, 5))]
+    scale = dh ** -0.5 if part == "v" else 2.0 ** 17
+    print("small", dtype, part, flush=True)
+    if part == "v" and dtype == "float16":       # (the result has its own smallest number)
+        q = q.float().bfloat16()
+    y, _ = check(gpu, c, q, table, lens, news, trees=trees, rows=some(news, 30), scale=scale)
+    assert (y != 0).any(axis=-1).all()
