@@ -918,31 +918,34 @@ def cache4_extend(page_table, lens, news, page_size, ring, ends, tokens, parents
     stride = page_table.stride(0)
     if batch > 1 and stride < pages:
         raise ValueError(f"{what}: page_table of strides {page_table.stride()} overlaps itself")
-    inputs = [("page_table", page_table, 4 * (stride * max(batch - 1, 0) + pages)), ("ring", ring, 4 * ring.shape[0]),
-              ("lens", lens, 4 * batch), ("news", news, 4 * batch), ("ends", ends, 16)]
     tree, words = None, 0
     if parents is not None:
         if max_new is None or max_new < 1:
             raise ValueError(f"{what}: parents need max_new")
         _plain(what, "parents", parents, torch.int32, (tokens,), dev)
-        inputs.append(("parents", parents, 4 * tokens))
         words = (int(max_new) + 63) // 64
-        tree = torch.empty((tokens, words), dtype=torch.int64, device=dev)
+        tree = ends.new_empty((tokens, words))
     # the two that are written lie apart from each other and from all that is read
-    spans = [(t.data_ptr(), size) for _, t, size in inputs]
-    for i, (at, size) in enumerate(spans[:2]):
-        for j, (other, length) in enumerate(spans[i + 1:]):
-            if at < other + length and other < at + size and size and length:
-                raise ValueError(f"{what}: {inputs[i][0]} and {inputs[i + 1 + j][0]} share memory")
-    starts = torch.empty(batch + 1, dtype=torch.int32, device=dev)
-    after = torch.empty(batch, dtype=torch.int32, device=dev)
-    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-    positions = torch.empty(tokens, dtype=torch.int32, device=dev)
-    left = torch.empty(2, dtype=torch.int64, device=dev)
+    at, size = page_table.data_ptr(), 4 * (stride * max(batch - 1, 0) + pages)
+    ring_at, ring_size = ring.data_ptr(), 4 * ring.shape[0]
+    if at < ring_at + ring_size and ring_at < at + size and size:
+        raise ValueError(f"{what}: page_table and ring share memory")
+    for name, t, length in (("lens", lens, 4 * batch), ("news", news, 4 * batch), ("ends", ends, 16),
+                            ("parents", parents, 4 * tokens)):
+        if t is None or not length:
+            continue
+        other = t.data_ptr()
+        if other < ring_at + ring_size and ring_at < other + length:
+            raise ValueError(f"{what}: ring and {name} share memory")
+        if other < at + size and at < other + length and size:
+            raise ValueError(f"{what}: page_table and {name} share memory")
+    # (of the inputs' types and device: less host time than torch.empty)
+    starts, after, positions = lens.new_empty(batch + 1), lens.new_empty(batch), lens.new_empty(tokens)
+    slots, left = ends.new_empty(tokens), ends.new_empty(2)
     size = _workspace_extend(batch)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    a = _lib.Extend4(spans[0][0], stride, pages, batch, lens.data_ptr(),
-                     news.data_ptr(), ring.data_ptr(), ring.shape[0], ends.data_ptr(), tokens,
+    a = _lib.Extend4(at, stride, pages, batch, lens.data_ptr(),
+                     news.data_ptr(), ring_at, ring.shape[0], ends.data_ptr(), tokens,
                      None if parents is None else parents.data_ptr(), words, starts.data_ptr(),
                      after.data_ptr(), slots.data_ptr(), positions.data_ptr(), left.data_ptr(),
                      None if tree is None else tree.data_ptr(), page_size,
