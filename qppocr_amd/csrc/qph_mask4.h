@@ -929,6 +929,10 @@ mask4_shared_kernel(Mask4 g) {
       const bool some = next_part(late_args(), at, end, part, parts);
       __syncthreads();                    // (the last part's reads of LDS too)
       if (!some) break;
+      // (in scalar registers, and with them all that follows from it: float32 trees of 32
+      // sequences 140 us, 201 where the compiler held them in each lane)
+      part = Part4{(int)same_in_all(part.b), (int)same_in_all(part.h), 0, (int)same_in_all(part.split),
+                   same_in_all(part.va), same_in_all(part.vb)};
       if (thread == 0) *state = EvenState{at, end, part};
       if (part.va == 0) unused_splits(late_args(), part, parts);
     } else {
