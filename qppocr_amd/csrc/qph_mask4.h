@@ -623,8 +623,17 @@ __device__ __forceinline__ void store_rows(const Attn4& a, const Walk4& w, const
 template <int NQ>
 constexpr int mask4_few_waves(int terms, int w) { return NQ == 1 && w <= 4 && terms < 3 ? 12 : 4; }
 
+// Waves a SIMD that the compiler keeps registers free for.  Two where it would take a few
+// past half of them by itself (bfloat16, heads of 128, 32 rows: 68 us, 88 without; of 192, 16
+// rows: 78 and 94); with more terms of such heads it would keep values in memory (float16 of
+// 256: 173 and 107, float32 of 192: 168 and 115).
+template <int NQ>
+constexpr int mask4_few_simd(int terms, int w) {
+  return mask4_few_waves<NQ>(terms, w) > 4 ? 3 : (terms < 3 && NQ == 2 && w == 4) || (terms == 1 && w >= 6) ? 2 : 1;
+}
+
 template <typename E, int W, int NQ>
-__global__ __launch_bounds__(64 * mask4_few_waves<NQ>(E::terms, W), mask4_few_waves<NQ>(E::terms, W) / 4) void
+__global__ __launch_bounds__(64 * mask4_few_waves<NQ>(E::terms, W), mask4_few_simd<NQ>(E::terms, W)) void
 mask4_few_kernel(Mask4 g) {
   const Attn4& a = g.a;
   constexpr int R = 16 * NQ;

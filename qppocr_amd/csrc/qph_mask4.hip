@@ -72,12 +72,11 @@ static int launch_mask4_join(const Attn4& a, int dh, hipStream_t s) {
 // How a call is split.  Up to 32 rows of a sequence and head take the few-row form.  Up to
 // 256 take it too while its workgroups all run at once and read little of the cache between
 // them: each decodes the keys of its 32 rows anew, which costs less than the many-row form's
-// longer way to its first product.  (32 query heads over 8; few-row against many-row form:
-// one sequence, 256 rows of 130 bfloat16 keys 13 and 22 us, of 4000 keys 36 and 47, of 16000
-// 74 and 58; eight sequences, 128 rows of 4000 keys 62 and 48; 24 sequences, 256 rows of 130
-// keys 53 and 24, 96 rows 21 and 20.  In float32, whose products
-// cost more than the decoding: eight sequences, 40 rows of 16000 keys 88 and 110 us, 128
-// rows 192 and 158.)
+// longer way to its first product.  (bfloat16, 32 query heads over 8; few-row against many-row
+// form: one sequence, 256 rows of 130 keys 14 and 22 us, of 4000 keys 32 and 49, of 16000 64
+// and 60; eight sequences, 128 rows of 4000 keys 50 and 54; 24 sequences, 96 rows of 1500 keys
+// 31 and 48, 256 rows of 130 keys 33 and 24.  float32: eight sequences, 40 rows of 16000 keys
+// 88 and 110 us, 128 rows 192 and 158.)
 static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_attn4_mask* mask) {
   Mask4Plan r{};
   const int64_t rows = std::min<int64_t>((int64_t)p->max_new * (p->heads / c->heads), 1 << 30);
@@ -88,8 +87,7 @@ static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_a
   const int terms = p->dtype == QPH_F32 ? 3 : 1, w = c->dh / 32;
   r.nq = rows > 16 ? mask4_nq(terms, w) : 1;
   int64_t tiles = (rows + 16 * r.nq - 1) / (16 * r.nq);
-  const bool few = rows <= 32 || (rows <= 256 && tiles * seqs <= 768 &&
-                                  tiles * seqs * keys <= (terms > 1 ? 1000000 : 400000));
+  const bool few = rows <= 32 || (rows <= 256 && tiles * seqs <= 768 && tiles * seqs * keys <= 1000000);
   if (!few) {
     const int64_t most = mask4_waves(terms, w);
     const int64_t groups = (tiles + most - 1) / most;
