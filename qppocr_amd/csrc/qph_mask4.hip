@@ -69,14 +69,17 @@ static int launch_mask4_join(const Attn4& a, int dh, hipStream_t s) {
   return launch_check("mask4_join_kernel");
 }
 
-// How a call is split.  Up to 32 rows of a sequence and head take the few-row form.  Up to
-// 256 take it too while its workgroups all run at once and read little of the cache between
-// them: each decodes the keys of its 32 rows anew, which costs less than the many-row form's
-// longer way to its first product.  (bfloat16, 32 query heads over 8; few-row against many-row
+// How a call is split.  Up to two tiles of rows of a sequence and head take the few-row form.
+// Up to 256 rows take it too while its workgroups all run at once and read little of the cache
+// between them: each decodes the keys of its 32 rows anew, which costs less than the many-row
+// form's longer way to its first product.  (bfloat16, 32 query heads over 8; few-row against many-row
 // form: one sequence, 256 rows of 130 keys 14 and 22 us, of 4000 keys 32 and 49, of 16000 64
 // and 60; eight sequences, 128 rows of 4000 keys 50 and 54; 24 sequences, 96 rows of 1500 keys
 // 31 and 48, 256 rows of 130 keys 33 and 24.  float32: eight sequences, 40 rows of 16000 keys
-// 88 and 110 us, 128 rows 192 and 158.)
+// 88 and 110 us, 128 rows 192 and 158.  Two tiles, heads of 128 and of 64 in float16, of 64 in
+// float32: 64 sequences, 64 rows of up to 4000 keys 124 and 147, 87 and 114, 106 and 130; 16
+// sequences, 48 rows of up to 16000 keys 101 and 131, 74 and 101, 87 and 119; bfloat16, 32
+// sequences, 64 rows of up to 8000 keys 120 and 110, of 96 elements 127 and 105.)
 static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_attn4_mask* mask) {
   Mask4Plan r{};
   const int64_t rows = std::min<int64_t>((int64_t)p->max_new * (p->heads / c->heads), 1 << 30);
@@ -87,7 +90,7 @@ static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_a
   const int terms = p->dtype == QPH_F32 ? 3 : 1, w = c->dh / 32;
   r.nq = rows > 16 ? mask4_nq(terms, w) : 1;
   int64_t tiles = (rows + 16 * r.nq - 1) / (16 * r.nq);
-  const bool few = rows <= 32 || (rows <= 256 && tiles * seqs <= 768 && tiles * seqs * keys <= 1000000);
+  const bool few = tiles <= 2 || (rows <= 256 && tiles * seqs <= 768 && tiles * seqs * keys <= 1000000);
   if (!few) {
     const int64_t most = mask4_waves(terms, w);
     const int64_t groups = (tiles + most - 1) / most;
