@@ -92,7 +92,9 @@ static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_a
   int64_t tiles = (rows + 16 * r.nq - 1) / (16 * r.nq);
   const bool few = tiles <= 2 || (rows <= 256 && tiles * seqs <= 768 && tiles * seqs * keys <= 1000000);
   if (!few) {
-    const int64_t most = mask4_waves(terms, w);
+    // (a launch has fewer than 2^32 threads: four waves a workgroup where eight of so many
+    // sequences' heads pass that)
+    const int64_t most = seqs <= (((int64_t)1 << 32) - 1) / 512 ? mask4_waves(terms, w) : 4;
     const int64_t groups = (tiles + most - 1) / most;
     r.waves = (int)std::max<int64_t>((tiles + groups - 1) / groups, 4);
     tiles = groups;
