@@ -764,8 +764,11 @@ template <> struct Shared4<BF16> { static constexpr int kterms = 1, pterms = 1; 
 constexpr float kHigh = 14.0f;
 
 // The scale byte of a block whose codes (this lane's word of them) are `codes`, for
-// float16: any for zeros.
-__device__ __forceinline__ unsigned f16_scale(unsigned s, unsigned codes) { return codes & 0x77777777u ? s : 127u; }
+// float16: any for zeros with a scale below its range.  (Past the range it stays, zeros or
+// not: a written block of NaN has the mark 255 and zeros for codes.)
+__device__ __forceinline__ unsigned f16_scale(unsigned s, unsigned codes) {
+  return s >= 104u || codes & 0x77777777u ? s : 127u;
+}
 
 __device__ __forceinline__ bool f16_holds(unsigned s) { return s - 104u <= 36u; }
 
