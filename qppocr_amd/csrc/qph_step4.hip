@@ -170,8 +170,10 @@ __device__ __forceinline__ unsigned ring_place(int64_t at, unsigned n) {
 // more than the few thousand additions.  A row's page comes from the table where
 // its sequence had the page before, and else from the ring, not from the entry
 // that another thread writes now.  Bound by trips to memory one after the other
-// (lengths, sums, a page, its entry, a parent): 48 trees of up to 32 tokens 8.4
-// us, 384 prompts of some 940000 tokens in all (11 MB) 12.8.
+// (lengths, sums, a page, its entry, a parent): 48 trees of up to 32 tokens 8.3
+// us, 384 prompts of some 940000 tokens in all (11 MB) 12.6.  A path is such a row of
+// trips as long as it is deep, 0.19 us each: 48 sequences of 32, 200 and 700 tokens 9,
+// 38 and 134 us as chains, 6.5, 7.4 and 9.2 as binary trees; one chain of 16384 3.2 ms.
 template <bool FEW>
 __global__ __launch_bounds__(256) void extend4_kernel(Extend4 a) {
   __shared__ int lds[FEW ? 3 * (kExtendFew + 1) : 1];
@@ -468,7 +470,7 @@ __device__ __forceinline__ int64_t move_block(const Move4& a, int64_t slot, unsi
 
 // A few tokens: a workgroup has all of them for its head's keys or values, reads
 // all, then writes all, so that a place may be left and taken in one call.  (190
-// tokens of 8 heads of 128: 2.7 us, a launch and three trips to memory.)
+// tokens of 8 heads of 128: 2.8 us, a launch and three trips to memory.)
 template <int U>
 __global__ __launch_bounds__(1024) void move4_few_kernel(Move4 a) {
   const unsigned h = blockIdx.x >> 1, second = blockIdx.x & 1;
@@ -526,7 +528,7 @@ __global__ __launch_bounds__(256) void move4_many_kernel(Move4 a) {
 
 // Blocks of a head that a workgroup holds in its registers (4 each of 1024 threads).
 static bool move4_few(const qph_cache4* c, int64_t tokens) {
-  return tokens <= 16 * 1024 && tokens * (c->dh / 32) <= 4 * 1024;
+  return tokens * (c->dh / 32) <= 4 * 1024;
 }
 
 static size_t move4_workspace(const qph_cache4* c, int64_t tokens) {
