@@ -432,10 +432,15 @@ QPH_API int qph_attention_cache4(qph_ctx* ctx, const qph_cache4* cache, const qp
  * context as the path is long).  A window hides no drafted token, causal is not
  * used, and bits from n on count for nothing.  tree_words is 0 without a tree and
  * max_new / 64 rounded up at least with one (drafted tokens past the words are not
- * seen).  Where a head has many rows, the probabilities of bfloat16 rows keep 11
- * bits before they meet the values, those of the others 21 and more.  The scales
- * are 4-byte aligned.  Everything else is as in qph_attention_cache4, the
- * workspace's rules too. */
+ * seen).  Before they meet the values, a row's probabilities are rounded by at most
+ * 2^-16 of themselves (float32: 2^-23), as in qph_attention_cache4, where a head has
+ * few rows.  Where it has many (how many goes by the sizes), bfloat16 rows' are by
+ * 2^-11 of themselves and float16 rows' by 2^-22, or by 2^-31 of the row's largest
+ * where that is more; there a block with a NaN or an infinity, or with numbers that
+ * float16 does not hold (scale bytes below 104 or above 140), has all rows of a
+ * workgroup that meets it computed a second and slower time.  The scales are 4-byte
+ * aligned.  Everything else is as in qph_attention_cache4, the workspace's rules
+ * too. */
 typedef struct {
   int64_t sinks;
   const uint64_t* tree;       /* [tokens][tree_words], device */
@@ -462,13 +467,19 @@ QPH_API int qph_attention_mask4(qph_ctx* ctx, const qph_cache4* cache, const qph
  * Sequences take pages in their order.  One whose pages are not all there, that
  * its row of the table does not hold or whose rows end past `tokens` is not
  * granted: its length stays, its rows' slots are -1 and it takes no page (nor does
- * any later one that needs some, where pages ran out).  page_table is written where
+ * any later one that needs some, where pages ran out).  Its rows stay in starts all
+ * the same: an attention takes the last of its cached tokens for them, so that what
+ * it answers for rows with slot -1 means nothing; out_lens less lens says on the
+ * device how many tokens each sequence was granted.  page_table is written where
  * pages are taken (entries behind a sequence's last page mean nothing), the ring
  * where they are given back.  parents[t] is the index of row t's parent among its
  * sequence's new tokens, smaller than its own; anything else makes it a child of
- * the context.  Rows of no sequence get slot -1, position 0 and no bits.  The
- * outputs share no memory with the inputs.  page_size is a power of two, 16 to
- * 32768.  workspace: qph_cache4_extend_workspace bytes, as for the attention. */
+ * the context.  Bits past the words are dropped.  A row's path is walked parent by
+ * parent, so that the time grows with the depth of the deepest one (0.19 us a
+ * token: a chain of 4096 takes 0.8 ms).  Rows of no sequence get slot -1, position 0
+ * and no bits.  The outputs share no memory with the inputs.  page_size is a power of
+ * two, 16 to 32768.  workspace: qph_cache4_extend_workspace bytes, as for the
+ * attention. */
 typedef struct {
   int32_t* page_table;        /* [batch][max_pages], rows table_stride apart */
   int64_t table_stride, max_pages, batch;
@@ -506,10 +517,11 @@ QPH_API int qph_cache4_move(qph_ctx* ctx, const qph_cache4* cache, const int64_t
  * turns[i] / 2^64 turns:
  *   (u, v) -> (u cos t - v sin t, u sin t + v cos t)
  * or with inverse by -t (the transpose, which is the gradient's rotation too).  The
- * product is exact modulo a turn.  Elements from 2 pairs on are copied.  x and out
- * [tokens][heads][dh] have strides {token, head}; out may be x itself (with its
- * strides) and shares no memory with it otherwise.  Cosines, sines and products are
- * float32, out is rounded once. */
+ * product is exact modulo a turn (a frequency rounded to 2^-64 turns is off by 2^-65
+ * of one a position: by 2^-34 of a turn at position 2^31).  Elements from 2 pairs on
+ * are copied.  x and out [tokens][heads][dh] have strides {token, head}; out may be x
+ * itself (with its strides) and shares no memory with it otherwise.  Cosines, sines
+ * and products are float32, out is rounded once. */
 typedef struct {
   const void* x;
   void* out;

@@ -113,9 +113,15 @@ static Mask4Plan mask4_plan(const qph_cache4* c, const qph_attn4* p, const qph_a
   int64_t n = 1;
   if (2 * blocks <= most && keys > 2 * least)
     n = std::min<int64_t>({most / blocks, (keys + least - 1) / least, 64});
-  // Three splits of few rows where a CU has one workgroup: twelve waves of it instead, without
-  // a join (32 sequences of 8 heads, windows of 4096: 36.8 us, 40.0 with splits).  Two splits
-  // are kept: eight waves a workgroup leave some CUs two (40 sequences: 58 us, 47 with splits).
+  // Three splits of few rows where a CU has one workgroup at most: twelve waves of it instead,
+  // the same number without the join's launch.  (One token, twelve waves against three splits:
+  // 32 sequences of 8 heads, windows of 4096 36.8 and 40.0 us; 25 sequences of 1100 keys, heads
+  // of 128 and 32 16.7 and 21.4, 11.0 and 15.0; 8 sequences of 16 heads of 700 keys, bfloat16
+  // 13.4 and 15.2, float16 14.8 and 16.4.  In up to 32 workgroups, whose splits have a CU each,
+  // heads of 128 lose up to 8 %: one sequence of one head of 700 keys 12.2 and 11.9, float16
+  // 13.3 and 12.3; smaller heads gain there too: of 64 10.2 and 10.6, of 32 9.5 and 10.3.)  Two
+  // splits are kept: eight waves a workgroup leave some CUs two (40 sequences: 58 us, 47 with
+  // splits).
   r.few = !r.waves && r.nq == 1 && n == 3 && blocks <= 256 ? mask4_few_waves<1>(terms, w) : 4;
   if (r.few > 4) n = 1;
   // Several sequences of one row tile each: even shares of all their keys, which the

@@ -781,6 +781,10 @@ def attention_cache4(q, cache, page_table, lens, scale, starts=None, max_new=Non
     sequence's first `sinks`.  out may be q itself, and shares no memory with it
     otherwise, nor its elements any.  A row that sees no key is zero; rows of no
     sequence keep what out holds.
+    With sinks beside a window the cache's scales must be 4-byte aligned (a cache4's
+    are), and where a head has many rows, bfloat16 rows meet the values with
+    probabilities of 11 bits in place of 16 (the bounds: qph_attention_mask4 in
+    include/qppocr_hip.h).
     Returns out, or (out, lse) with the sums' logarithms, float32 [tokens,
     heads] (-infinity where no key is seen; a new tensor's rows of no sequence
     are undefined)."""
@@ -796,7 +800,10 @@ def attention_tree4(q, cache, page_table, lens, scale, tree, starts=None, max_ne
     makes such masks from parents).  Of the context (the cached tokens before the
     new ones) a token sees all, or with a window what that and the sinks leave of
     it for the end of its path, which stands as many places behind the context as
-    it has bits.  64 words must cover max_new."""
+    it has bits.  Words of 64 bits must cover max_new.  The scales' alignment and the
+    bits of the probabilities are as with sinks.  Rows that cache4_extend did not
+    grant (their slots are -1) are answered from other tokens' keys: what they get
+    means nothing."""
     what = "attention_tree4"
     if tree.dim() != 2 or tree.shape[0] != q.shape[0] or not tree.shape[1]:
         raise ValueError(f"{what}: tree int64 [{q.shape[0]}, words], not {tuple(tree.shape)}")
@@ -896,10 +903,13 @@ def cache4_extend(page_table, lens, news, page_size, ring, ends, tokens, parents
     slots (for cache4_write) and positions (for rotary).  lens and ends are those after
     the step.  A sequence whose pages are not all there, that its row of the table does
     not hold or whose rows end past `tokens` is not granted: its length stays and its
-    slots are -1.  With parents, int32 [tokens], the new tokens are drafted trees:
+    slots are -1 (Step4.lens less lens says how many tokens each was granted, or gave
+    back); its rows stay in starts, and what an attention answers for them means
+    nothing.  With parents, int32 [tokens], the new tokens are drafted trees:
     parents[t] is the index of a row's parent among its sequence's new ones, smaller
     than its own (else the context's), positions go by depth, and tree has
-    attention_tree4's masks for up to max_new (needed then) new tokens a sequence."""
+    attention_tree4's masks for up to max_new (needed then) new tokens a sequence.
+    Paths are walked parent by parent: 0.19 us for each token of the deepest."""
     what = "cache4_extend"
     if page_table.dim() != 2 or page_table.dtype != torch.int32 or (
             page_table.stride(1) != 1 and page_table.shape[1] > 1 and page_table.numel()):
@@ -1011,7 +1021,8 @@ _TWO_PI = fractions.Fraction(628318530717958647692528676655900576839433879875021
 
 def rotary_plan(dh, freqs, axes=None, neighbours=False, device="cuda"):
     """The Rotary of heads of dh elements whose pair i turns by freqs[i] radians a
-    position (numbers; usually base^(-i / pairs)) of axis axes[i] (default: 0)."""
+    position (numbers; usually base^(-i / pairs)) of axis axes[i] (default: 0).  A
+    frequency is rounded to 2^-64 turns, which at position p is off by p 2^-65 turns."""
     freqs = [float(f) for f in freqs]
     axes = [0] * len(freqs) if axes is None else [int(a) for a in axes]
     if len(axes) != len(freqs) or not freqs or 2 * len(freqs) > dh:
