@@ -472,7 +472,8 @@ QPH_API int qph_attention_mask4(qph_ctx* ctx, const qph_cache4* cache, const qph
  * it answers for rows with slot -1 means nothing; out_lens less lens says on the
  * device how many tokens each sequence was granted.  page_table is written where
  * pages are taken (entries behind a sequence's last page mean nothing), the ring
- * where they are given back.  parents[t] is the index of row t's parent among its
+ * where they are given back.  Sequences share no pages here: one that stands in two
+ * rows of the table is given back by each of them.  parents[t] is the index of row t's parent among its
  * sequence's new tokens, smaller than its own; anything else makes it a child of
  * the context.  Bits past the words are dropped.  A row's path is walked parent by
  * parent, so that the time grows with the depth of the deepest one (0.19 us a

@@ -896,8 +896,9 @@ def cache4_extend(page_table, lens, news, page_size, ring, ends, tokens, parents
     shrinks by -news[b].  Free pages are ring[i % len(ring)] (int32) for ends[0] <= i <
     ends[1] (int64 [2]); a ring with room for every page of the pool never runs over.
     page_table and the ring are written in place: pages that sequences take, in their
-    order, and pages that they give back, which the next call can take.  The entries
-    behind a sequence's last page mean nothing.
+    order, and pages that they give back, which the next call can take (a page that two
+    rows share is given back by each).  The entries behind a sequence's last page mean
+    nothing.
 
     Of the step's rows, `tokens` in all, sequence b has starts[b] to starts[b + 1]: their
     slots (for cache4_write) and positions (for rotary).  lens and ends are those after
